@@ -1,0 +1,493 @@
+"""The operators around a draft tree over the paged, quantized cache, as cases that can be timed and compared.
+
+A case is one call on one stream: the normed and rotated append of new tokens (queries out, keys and values quantized into
+their pages), the attention of a tree of drafted tokens over the cache, the log probabilities, entropy and best alternatives of
+rows of logits, or the copy of cache rows (an accepted path moved together, a fork's page filled). With `own` false the
+same is computed from elementary torch operations.
+"""
+import math
+
+import torch
+
+own = False
+
+PAGE = 4096                                           # keys per page
+BLOCK = {"f16": 64, "q8_0": 34, "q4_0": 18}           # bytes per 32 values
+FMT = {"f16": 0, "q8_0": 1, "q4_0": 2}
+TYPE = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+SIZE = {"f32": 4, "f16": 2, "bf16": 2}
+
+
+# ---------------------------------------------------------------- cases
+def _append(name, fmt, dtype, heads, gqa, hd, rot, tokens, pos, tree=False, interleaved=False):
+    return {"name": name, "op": "append", "fmt": fmt, "type": dtype, "heads": heads, "gqa": gqa, "hd": hd, "rot": rot,
+            "tokens": tokens, "pos": pos, "tree": tree, "interleaved": interleaved}
+
+
+def _tree(name, fmt, heads, gqa, hd, nodes, keys, page=PAGE):
+    return {"name": name, "op": "tree", "fmt": fmt, "heads": heads, "gqa": gqa, "hd": hd, "nodes": nodes, "keys": keys, "page": page}
+
+
+def _logprobs(name, dtype, rows, vocab, given, top, scale=1.0, pad=0):
+    return {"name": name, "op": "logprobs", "type": dtype, "rows": rows, "vocab": vocab, "given": given, "top": top, "scale": scale,
+            "pad": pad}
+
+
+def _copy(name, kind, fmt, layers, heads, hd, rows, page):
+    return {"name": name, "op": "copy", "kind": kind, "fmt": fmt, "layers": layers, "heads": heads, "hd": hd, "rows": rows, "page": page}
+
+
+def listed():
+    return [
+        # one new token of a decode step at a far position, 64 query and 8 KV heads: launch and latency
+        _append("append 1 token q8_0", "q8_0", "f32", 8, 8, 128, 128, 1, 131071),
+        # a tree of 26 drafted tokens (siblings share a position), a quarter of each head of 256 rotated
+        _append("append 26 nodes q4_0 bf16", "q4_0", "bf16", 4, 6, 256, 64, 26, 3990, tree=True),
+        # a long prefill chunk from a bf16 projection
+        _append("append 2048 tokens q8_0 bf16", "q8_0", "bf16", 8, 8, 128, 128, 2048, 3900),
+        # the plain next token after 4k keys: the smallest tree
+        _tree("tree 1 node 4k q8_0", "q8_0", 8, 8, 128, 1, 4097),
+        # a tree of 26 over a 4-bit cache that ends inside a page and inside a tile
+        _tree("tree 26 nodes 33k q4_0", "q4_0", 8, 8, 128, 26, 33333),
+        # a wide tree over a long cache: the largest call
+        _tree("tree 64 nodes 96k q8_0", "q8_0", 8, 8, 128, 64, 98304),
+        # 8 nodes at 6 query heads per KV head of 256
+        _tree("tree head 256 64k q8_0", "q8_0", 4, 6, 256, 8, 65536),
+        # one sampled token with its alternatives
+        _logprobs("logprobs 1 row f32", "f32", 1, 151936, 1, 5),
+        # the nodes of a draft tree, each with its children's tokens, at a temperature
+        _logprobs("logprobs 27 rows f32", "f32", 27, 151936, 4, 8, scale=1.25),
+        # scoring a prompt: one given token per row, many rows of half-width logits in a padded matrix
+        _logprobs("logprobs 512 rows bf16", "bf16", 512, 128256, 1, 20, pad=64),
+        # the accepted path of 7 nodes moved together in every layer
+        _copy("keep 7 rows 64 layers q8_0", "keep", "q8_0", 64, 8, 128, 7, 256),
+        # a fork takes its own copy of a partly filled page in every layer
+        _copy("fork 2219 rows 64 layers q8_0", "fork", "q8_0", 64, 8, 128, 2219, PAGE),
+    ]
+
+
+def _log(rng, lo, hi):
+    return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+
+def draw(rng):
+    op = rng.choice(["append", "tree", "tree", "tree", "logprobs", "logprobs", "copy"])
+    fmt = rng.choice(["q8_0", "q8_0", "q4_0", "f16"])
+    hd = rng.choice([128, 128, 256])
+    heads, gqa = rng.choice([(8, 8), (8, 4), (2, 7), (8, 5)] if hd == 128 else [(4, 6), (2, 8)])
+    if op == "append":
+        tree = rng.random() < 0.4
+        return {"op": op, "fmt": fmt, "type": rng.choice(["f32", "f16", "bf16"]), "heads": heads, "gqa": gqa, "hd": hd,
+                "rot": rng.choice([hd, hd, hd // 2, hd // 4]), "tokens": rng.randint(2, 64) if tree else _log(rng, 1, 1024),
+                "pos": _log(rng, 1, 1000000), "tree": tree, "interleaved": rng.random() < 0.4}
+    if op == "tree":
+        nodes = rng.choice([1, rng.randint(2, 16), rng.randint(17, 64)])
+        return {"op": op, "fmt": fmt, "heads": heads, "gqa": gqa, "hd": hd, "nodes": nodes,
+                "keys": nodes + _log(rng, 100, 48000 if fmt == "f16" else 96000), "page": rng.choice([PAGE, PAGE, 1000])}
+    if op == "logprobs":
+        rows = _log(rng, 1, 400)
+        return {"op": op, "type": rng.choice(["f32", "f16", "bf16"]), "rows": rows,
+                "vocab": _log(rng, 1000, min(262144, 30000000 // rows)), "given": rng.randint(1, 8), "top": rng.randint(0, 32),
+                "scale": rng.choice([1.0, 0.5, 1.25]), "pad": rng.choice([0, 0, rng.randint(1, 200)])}
+    if rng.random() < 0.5:
+        return {"op": op, "kind": "keep", "fmt": fmt, "layers": rng.randint(1, 64), "heads": heads, "hd": hd,
+                "rows": rng.randint(1, 48), "page": 256}
+    return {"op": op, "kind": "fork", "fmt": fmt, "layers": rng.randint(1, 32), "heads": heads, "hd": hd,
+            "rows": _log(rng, 1, 2000), "page": PAGE}
+
+
+# ---------------------------------------------------------------- inputs
+def _quantize(x, fmt):
+    """fp32 [n, 32] -> block bytes [n, 34 / 18 / 64] by ggml's reference rules, every operation rounded as written. (Divisors are
+    tensors: a division by a number may become a product with its reciprocal.)"""
+    if fmt == "f16":
+        return x.half().view(torch.uint8)
+    a = x.abs()
+    if fmt == "q8_0":
+        d = a.amax(1, keepdim=True) / torch.full((1, 1), 127.0, device=x.device)
+        r = torch.where(d != 0, torch.ones_like(d) / d, torch.zeros_like(d))
+        t = (x * r).double()
+        q = (torch.sign(t) * torch.floor(t.abs() + 0.5)).to(torch.int8).view(torch.uint8)
+        return torch.cat([d.half().view(torch.uint8), q], 1)
+    place = torch.arange(32, device=x.device)
+    first = 31 - torch.where(a == a.amax(1, keepdim=True), 31 - place, -1).amax(1, keepdim=True)
+    d = x.gather(1, first) * -0.125                                   # a power of two: exact
+    r = torch.where(d != 0, torch.ones_like(d) / d, torch.zeros_like(d))
+    q = (x * r + 8.5).to(torch.int32).clamp(0, 15).to(torch.uint8)
+    return torch.cat([d.half().view(torch.uint8), q[:, :16] | (q[:, 16:] << 4)], 1)
+
+
+def _rows(gen, keys, heads, hd, fmt, outliers):
+    """K or V rows of N(0,1) values, as bytes [keys, heads * head bytes]; K with 4 channels per head scaled by 8, the outlier
+    channels of real keys."""
+    out = torch.empty(keys, heads * hd // 32 * BLOCK[fmt], dtype=torch.uint8, device="cuda")
+    gain = torch.ones(heads, hd, device="cuda")
+    if outliers:
+        at = torch.rand(heads, hd, generator=gen, device="cuda").argsort(1)[:, :4]
+        gain.scatter_(1, at, 8.0)
+    for k0 in range(0, keys, 16384):
+        n = min(16384, keys - k0)
+        x = torch.randn(n, heads, hd, generator=gen, device="cuda") * gain
+        out[k0:k0 + n] = _quantize(x.reshape(-1, 32), fmt).reshape(n, -1)
+    return out
+
+
+def _parents(seed, n):
+    """A random tree: node 0 is its root, every other node's parent comes before it."""
+    gen = torch.Generator().manual_seed(seed)
+    u = torch.rand(n, generator=gen).tolist()
+    return [-1] + [int((0.3 + 0.7 * u[i]) * i) for i in range(1, n)]
+
+
+def _held(rows, fmt, heads, hd):
+    """The row bytes [n, rs] as what they hold, without a copy: {"d": the blocks' f16 scales, "q": their quants (q8_0: signed
+    numbers; q4_0: two nibbles each)}, or {"x": f16 values}."""
+    if fmt == "f16":
+        return {"x": rows.view(torch.float16)}
+    b = rows.unflatten(1, (heads * (hd // 32), BLOCK[fmt]))
+    q = b[..., 2:]
+    return {"d": b[..., :2].view(torch.float16), "q": q.view(torch.int8) if fmt == "q8_0" else q}
+
+
+def prepare(case, seed):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    s = {"case": case}
+    if case["op"] == "logprobs":
+        n, vocab, width = case["rows"], case["vocab"], case["vocab"] + case["pad"]
+        x = torch.randn(n, width, generator=gen, device="cuda") * 2.5
+        lead = torch.randint(0, vocab, (n, 6), generator=gen, device="cuda")     # a few likely tokens, some rows sure of one
+        x.scatter_add_(1, lead, torch.rand(n, 6, generator=gen, device="cuda") * 16.0)
+        banned = torch.randint(0, vocab, (max(1, vocab // 500),), generator=gen, device="cuda")
+        x[:, banned] = -math.inf                                                 # tokens that the sampler forbids
+        s["logits"] = x.to(TYPE[case["type"]])
+        ids = torch.randint(0, vocab, (n, case["given"]), generator=gen, device="cuda")
+        ids[:, 0] = lead[:, 0]
+        s["ids"] = ids.to(torch.int32)
+        f = lambda *shape: torch.zeros(*shape, device="cuda")  # noqa: E731
+        s["out"] = {"logp": f(n, case["given"]), "lse": f(n), "entropy": f(n)}
+        if case["top"]:
+            s["out"] |= {"top": torch.zeros(n, case["top"], dtype=torch.int32, device="cuda"), "top_logp": f(n, case["top"])}
+        return s
+    heads, hd, fmt = case["heads"], case["hd"], case["fmt"]
+    row = heads * hd // 32 * BLOCK[fmt]
+    if case["op"] == "copy":
+        n, page, layers = case["rows"], case["page"], case["layers"]
+        data = torch.randint(0, 256, (layers, 2, page, row), generator=gen, device="cuda", dtype=torch.uint8)
+        if case["kind"] == "keep":
+            # n accepted nodes of a tree whose rows begin inside the page: the root stays, later ones lie ever further apart
+            hops = torch.randint(1, 4, (n,), generator=torch.Generator().manual_seed(seed)).cumsum(0)
+            base = page // 4
+            s["from"], s["to"] = [base + int(h) - int(hops[0]) for h in hops], base
+            s["src"] = s["dst"] = data
+        else:
+            s["from"], s["to"] = range(n), 0
+            s["src"], s["dst"] = data, torch.zeros_like(data)
+        return s
+    gqa = case["gqa"]
+    if case["op"] == "append":
+        n, rot = case["tokens"], case["rot"]
+        wide = (heads * gqa + 2 * heads) * hd
+        s["qkv"] = torch.randn(n, wide, generator=gen, device="cuda").to(TYPE[case["type"]])  # one projection's output
+        s["qw"] = 1.0 + 0.2 * torch.randn(hd, generator=gen, device="cuda")
+        s["kw"] = 1.0 + 0.2 * torch.randn(hd, generator=gen, device="cuda")
+        s["freq"] = (1e6 ** (-2.0 * torch.arange(rot // 2, dtype=torch.float64) / rot)).float().cuda()
+        depth = list(range(n))
+        if case["tree"]:
+            depth = [0] * n
+            for i, p in enumerate(_parents(seed, n)):
+                depth[i] = depth[p] + 1 if p >= 0 else 0
+        s["positions"] = (case["pos"] + torch.tensor(depth)).to(torch.int32).cuda()
+        s["at"] = case["pos"] % (2 * PAGE)                           # where in the held pages the new rows go
+        keys = (s["at"] + n + PAGE - 1) // PAGE * PAGE
+        s["k"] = torch.zeros(keys, row, dtype=torch.uint8, device="cuda")
+        s["v"] = torch.zeros_like(s["k"])
+        s["q"] = torch.zeros(heads, gqa * n, hd, device="cuda")
+        k, v = (_held(s[t][s["at"]:s["at"] + n], fmt, heads, hd) for t in ("k", "v"))
+        s["out"] = {"q": s["q"], "k": k, "v": v}
+        return s
+    n = case["nodes"]
+    s["k"] = _rows(gen, case["keys"], heads, hd, fmt, True)
+    s["v"] = _rows(gen, case["keys"], heads, hd, fmt, False)
+    s["q"] = torch.randn(heads, gqa * n, hd, generator=gen, device="cuda")
+    mask = []
+    for i, p in enumerate(_parents(seed, n)):
+        mask.append((mask[p] if p >= 0 else 0) | 1 << i)
+    s["mask"] = torch.tensor([m - (m >> 63 << 64) for m in mask], dtype=torch.int64, device="cuda")
+    s["out"] = {"o": torch.zeros(heads, gqa * n, hd, dtype=torch.float16, device="cuda"), "lse": torch.zeros(heads, gqa * n, device="cuda")}
+    return s
+
+
+# ---------------------------------------------------------------- the framework's calls
+_ws = None
+
+
+def _handles(s):
+    """What a serving loop keeps beside its tensors: the workspace of its stream, the page tables, the call's shape."""
+    global _ws
+    import backburner_amd as bb
+    if _ws is None:
+        _ws = bb.Workspace()
+    case = s["case"]
+    h = {"bb": bb, "ws": _ws, "stream": torch.cuda.current_stream().cuda_stream}
+    if case["op"] == "logprobs":
+        h["type"] = {"f32": bb.TYPE_F32, "f16": bb.TYPE_F16, "bf16": bb.TYPE_BF16}[case["type"]]
+        return h
+    heads, hd, fmt = case["heads"], case["hd"], FMT[case["fmt"]]
+    if case["op"] == "copy":
+        h["shape"] = bb.make_shape(heads, 1, hd, fmt)
+        table = lambda x: bb.LayerTable([bb.Pages([l[0].data_ptr()], [l[1].data_ptr()], [case["page"]], []) for l in x])  # noqa: E731
+        h["src"] = table(s["src"])
+        h["dst"] = h["src"] if s["dst"] is s["src"] else table(s["dst"])
+        return h
+    n = case["tokens"] if case["op"] == "append" else case["nodes"]
+    h["shape"] = bb.make_shape(heads, case["gqa"] * n, hd, fmt)
+    rs, page, keys = h["shape"].rs, case.get("page", PAGE), s["k"].shape[0]
+    at = range(0, keys, page)
+    h["pages"] = bb.PageTable(bb.Pages([s["k"].data_ptr() + i * rs for i in at], [s["v"].data_ptr() + i * rs for i in at],
+                                       [min(page, keys - i) for i in at], []))
+    if case["op"] == "append":
+        wide = s["qkv"].shape[1]
+        h["rope"] = bb.make_rope(s["qw"].data_ptr(), s["kw"].data_ptr(), 1e-6, s["freq"].data_ptr(), case["rot"],
+                                 interleaved=case["interleaved"],
+                                 type={"f32": bb.TYPE_F32, "f16": bb.TYPE_F16, "bf16": bb.TYPE_BF16}[case["type"]],
+                                 q_stride=wide, k_stride=wide, v_stride=wide)
+        e = s["qkv"].element_size()
+        h["inputs"] = [s["qkv"].data_ptr() + e * hd * i for i in (0, heads * case["gqa"], heads * case["gqa"] + heads)]
+    return h
+
+
+def _run_own(s):
+    if "own" not in s:
+        s["own"] = _handles(s)
+    h, case = s["own"], s["case"]
+    bb, ws, st = h["bb"], h["ws"], h["stream"]
+    if case["op"] == "tree":
+        ws.attn_tree(h["shape"], h["pages"], case["nodes"], s["mask"].data_ptr(), s["q"].data_ptr(), s["out"]["o"].data_ptr(),
+                     s["out"]["lse"].data_ptr(), st)
+        return s["out"]
+    if case["op"] == "append":
+        q, k, v = h["inputs"]
+        bb.append_rope(h["shape"], h["pages"], PAGE, s["at"], h["rope"], q, k, v, s["positions"].data_ptr(), case["tokens"],
+                       s["q"].data_ptr(), st)
+        return s["out"]
+    if case["op"] == "logprobs":
+        o = s["out"]
+        ws.logprobs(s["logits"].data_ptr(), h["type"], case["rows"], case["vocab"], s["logits"].shape[1], case["scale"],
+                    s["ids"].data_ptr(), case["given"], case["top"], o["logp"].data_ptr(), o["lse"].data_ptr(), o["entropy"].data_ptr(),
+                    o["top"].data_ptr() if case["top"] else None, o["top_logp"].data_ptr() if case["top"] else None, st)
+        return o
+    bb.copy_rows(h["shape"], h["src"], h["dst"], case["page"], s["from"], s["to"], st)
+    return s["dst"]
+
+
+# ---------------------------------------------------------------- the plain forms
+def _values(rows, fmt, heads, hd):
+    """Row bytes [n, rs] as fp32 values [heads, n, hd]."""
+    n = rows.shape[0]
+    if fmt == "f16":
+        x = rows.view(torch.float16).float()
+    else:
+        b = rows.unflatten(1, (heads * (hd // 32), BLOCK[fmt]))
+        q = b[..., 2:]
+        q = q.view(torch.int8).float() if fmt == "q8_0" else torch.cat([q & 15, q >> 4], -1).float() - 8.0
+        x = b[..., :2].view(torch.float16).float() * q
+    return x.reshape(n, heads, hd).transpose(0, 1).contiguous()
+
+
+def _query(q, fmt):
+    """The query rounding of the call (part of its definition): q8_0 per 32 values over quantized keys, f16 over f16 keys."""
+    if fmt == "f16":
+        return q.half().float()
+    b = _quantize(q.reshape(-1, 32), "q8_0")
+    return (b[:, :2].view(torch.float16).float() * b[:, 2:].view(torch.int8).float()).reshape(q.shape)
+
+
+def _visible(mask, nodes, rows):
+    """[rows, nodes]: row g * nodes + t sees drafted key j where bit j of mask[t] is set."""
+    bits = (mask[:, None] >> torch.arange(nodes, device=mask.device)) & 1
+    return bits.bool().repeat(rows // nodes, 1)
+
+
+def _plain_tree(s):
+    case = s["case"]
+    fmt, heads, hd, n = case["fmt"], case["heads"], case["hd"], case["nodes"]
+    K, V = _values(s["k"], fmt, heads, hd), _values(s["v"], fmt, heads, hd)
+    S = torch.bmm(_query(s["q"], fmt), K.transpose(1, 2).contiguous()) * (1.0 / math.sqrt(hd))
+    S[:, :, -n:] = torch.where(_visible(s["mask"], n, S.shape[1]), S[:, :, -n:], -math.inf)
+    m = S.amax(2, keepdim=True)
+    P = torch.exp(S - torch.where(torch.isinf(m), 0.0, m))
+    l = P.sum(2, keepdim=True)
+    o = torch.bmm(P, V) / torch.where(l > 0, l, 1.0)
+    return {"o": o.half(), "lse": (m + torch.log(l)).squeeze(2)}
+
+
+def _plain_norm_rope(x, w, freq, positions, interleaved):
+    """[n, heads, hd] -> the same normed and rotated. In 64 bits: the angles of far positions need them, and the keys' next
+    step is a quantizer whose borders a last bit of 32 would cross."""
+    x = x.double()
+    y = x / torch.sqrt((x * x).mean(2, keepdim=True) + 1e-6) * w.double()
+    half = freq.numel()
+    th = (positions.double()[:, None] * freq.double())[:, None]
+    c, t = torch.cos(th), torch.sin(th)
+    if interleaved:
+        a, b = y[..., 0:2 * half:2], y[..., 1:2 * half:2]
+        r = torch.stack([a * c - b * t, a * t + b * c], 3).flatten(2)
+    else:
+        a, b = y[..., :half], y[..., half:2 * half]
+        r = torch.cat([a * c - b * t, a * t + b * c], 2)
+    return torch.cat([r, y[..., 2 * half:]], 2).float()
+
+
+def _plain_append(s):
+    case = s["case"]
+    n, heads, gqa, hd, fmt = case["tokens"], case["heads"], case["gqa"], case["hd"], case["fmt"]
+    q, k, v = (x.unflatten(1, (-1, hd)) for x in s["qkv"].split([heads * gqa * hd, heads * hd, heads * hd], 1))
+    q = _plain_norm_rope(q, s["qw"], s["freq"], s["positions"], case["interleaved"])
+    k = _plain_norm_rope(k, s["kw"], s["freq"], s["positions"], case["interleaved"])
+    rows = [_quantize(x.float().reshape(-1, 32), fmt).reshape(n, -1) for x in (k, v)]
+    return {"q": q.reshape(n, heads, gqa, hd).permute(1, 2, 0, 3).reshape(heads, gqa * n, hd).contiguous(),
+            "k": _held(rows[0], fmt, heads, hd), "v": _held(rows[1], fmt, heads, hd)}
+
+
+def _plain_logprobs(s):
+    case = s["case"]
+    x = s["logits"][:, :case["vocab"]].float()
+    y = x * case["scale"]
+    m = y.amax(1, keepdim=True)
+    e = torch.exp(y - m)
+    z = e.sum(1, keepdim=True)
+    lse = m + torch.log(z)
+    h = torch.log(z) - torch.where(e > 0, e * (y - m), 0.0).sum(1, keepdim=True) / z
+    out = {"logp": y.gather(1, s["ids"].long()) - lse, "lse": lse[:, 0], "entropy": h[:, 0]}
+    if case["top"]:
+        v, i = torch.sort(x, dim=1, descending=True, stable=True)
+        out |= {"top": i[:, :case["top"]].to(torch.int32), "top_logp": v[:, :case["top"]] * case["scale"] - lse}
+    return out
+
+
+def _plain_copy(s):
+    at = s["from"]
+    at = slice(at.start, at.stop) if isinstance(at, range) else torch.tensor(at, device="cuda")
+    s["dst"][:, :, s["to"]:s["to"] + len(s["from"])] = s["src"][:, :, at]
+    return s["dst"]
+
+
+def run(s):
+    if own:
+        return _run_own(s)
+    op = s["case"]["op"]
+    return _plain_tree(s) if op == "tree" else _plain_append(s) if op == "append" else _plain_logprobs(s) if op == "logprobs" else _plain_copy(s)
+
+
+def work(case):
+    if case["op"] == "logprobs":
+        n, values = case["rows"], case["rows"] * case["vocab"]
+        return {"bytes": SIZE[case["type"]] * values + n * (8 * case["given"] + 8 * case["top"] + 8), "flops": 5 * values}
+    row = case["heads"] * case["hd"] // 32 * BLOCK[case["fmt"]]
+    if case["op"] == "copy":
+        return {"bytes": 4 * case["layers"] * case["rows"] * row, "flops": 0}
+    heads, hd = case["heads"], case["hd"]
+    if case["op"] == "append":
+        n = case["tokens"]
+        q, kv = n * heads * case["gqa"] * hd, n * heads * hd
+        return {"bytes": SIZE[case["type"]] * (q + 2 * kv) + 4 * q + 2 * n * row, "flops": 10 * (q + kv) + 4 * kv}
+    rows = heads * case["gqa"] * case["nodes"]
+    return {"bytes": 2 * case["keys"] * row + 4 * rows * hd + rows * (2 * hd + 4), "flops": 4 * rows * case["keys"] * hd}
+
+
+# ---------------------------------------------------------------- the definitions in 64 bits
+def _exact_values(rows, fmt, heads, hd, h):
+    b = rows.reshape(rows.shape[0], heads, hd // 32, BLOCK[fmt])[:, h].contiguous()
+    if fmt == "f16":
+        return b.view(torch.float16).double().reshape(-1, hd)
+    d, q = b[..., :2].contiguous().view(torch.float16).double(), b[..., 2:].contiguous()
+    if fmt == "q8_0":
+        q = q.view(torch.int8).double()
+    else:
+        q = torch.stack([q % 16, q // 16], 2).reshape(*q.shape[:2], 32).double() - 8.0
+    return (d * q).reshape(-1, hd)
+
+
+def _exact_tree(case, s):
+    fmt, heads, hd, n, keys = case["fmt"], case["heads"], case["hd"], case["nodes"], case["keys"]
+    rows, bits = case["gqa"] * n, s["mask"].tolist()
+    sees = torch.tensor([[bits[r % n] >> j & 1 for j in range(n)] for r in range(rows)], dtype=torch.bool, device="cuda")
+    o = torch.zeros(heads, rows, hd, dtype=torch.float64, device="cuda")
+    lse = torch.zeros(heads, rows, dtype=torch.float64, device="cuda")
+    for h in range(heads):
+        q = s["q"][h].double()
+        if fmt == "f16":
+            q = s["q"][h].to(torch.float16).double()
+        else:
+            x = s["q"][h].reshape(-1, 32)
+            big = x.abs().max(1, keepdim=True).values
+            d = torch.div(big, torch.full_like(big, 127.0))
+            t = (x * torch.where(d > 0, torch.reciprocal(d), d)).double()
+            q = (torch.trunc(t + torch.copysign(torch.full_like(t, 0.5), t)) * d.to(torch.float16).double()).reshape(rows, hd)
+        m = torch.full((rows,), -math.inf, dtype=torch.float64, device="cuda")
+        l, acc = torch.zeros_like(m), o[h]
+        for k0 in range(0, keys, 16384):
+            k1 = min(keys, k0 + 16384)
+            z = q @ _exact_values(s["k"][k0:k1], fmt, heads, hd, h).t().contiguous() / math.sqrt(hd)
+            lo = max(k0, keys - n)
+            if lo < k1:
+                part = z[:, lo - k0:]
+                part[~sees[:, lo - (keys - n):k1 - (keys - n)]] = -math.inf
+            new = torch.maximum(m, z.max(1).values)
+            w = torch.exp(m - new)
+            p = torch.exp(z - new[:, None])
+            acc.mul_(w[:, None]).add_(p @ _exact_values(s["v"][k0:k1], fmt, heads, hd, h))
+            l, m = l * w + p.sum(1), new
+        acc.div_(l[:, None])
+        lse[h] = m + l.log()
+    return {"o": o, "lse": lse}
+
+
+def _exact_append(case, s):
+    """The rotated queries; the keys' scales and f16 keys by their formula (the quants are whole numbers)."""
+    n, heads, gqa, hd, rot, fmt = (case[k] for k in ("tokens", "heads", "gqa", "hd", "rot", "fmt"))
+    x = s["qkv"].cpu().double().reshape(n, -1, hd)
+    angle = s["positions"].cpu().double().reshape(n, 1, 1) * s["freq"].cpu().double().reshape(1, 1, -1)
+    turn = torch.polar(torch.ones_like(angle), angle)
+
+    def formula(x, w):
+        y = x * w.cpu().double() * (x.square().sum(-1, keepdim=True) / hd + 1e-6).rsqrt()
+        first, second = (slice(0, rot, 2), slice(1, rot, 2)) if case["interleaved"] else (slice(0, rot // 2), slice(rot // 2, rot))
+        z = torch.complex(y[..., first], y[..., second]) * turn
+        y[..., first], y[..., second] = z.real, z.imag
+        return y
+
+    def scales(y):
+        if fmt == "f16":
+            return {"x": y.reshape(n, -1)}
+        b = y.reshape(n, -1, 32)
+        if fmt == "q8_0":
+            return {"d": (b.abs().amax(2, keepdim=True) / 127.0), "q": None}
+        return {"d": b.gather(2, b.abs().argmax(2, keepdim=True)) / -8.0, "q": None}
+
+    q = formula(x[:, :heads * gqa].clone(), s["qw"])
+    k = formula(x[:, heads * gqa:heads * gqa + heads].clone(), s["kw"])
+    rows = [q[:, h * gqa + g] for h in range(heads) for g in range(gqa)]
+    return {"q": torch.stack(rows).reshape(heads, gqa * n, hd), "k": scales(k), "v": scales(x[:, heads * gqa + heads:].clone())}
+
+
+def _exact_logprobs(case, s):
+    out = {"logp": [], "lse": [], "entropy": [], "top_logp": []}
+    for r in range(case["rows"]):
+        y = s["logits"][r, :case["vocab"]].double() * case["scale"]
+        lse = torch.logsumexp(y, 0)
+        lp = y - lse
+        out["lse"].append(lse)
+        out["logp"].append(lp[s["ids"][r].long()])
+        out["entropy"].append(-(lp.exp() * torch.where(lp > -math.inf, lp, 0.0)).sum())
+        if case["top"]:
+            out["top_logp"].append(torch.topk(lp, case["top"]).values)
+    got = {k: torch.stack(v) for k, v in out.items() if v}
+    return got | ({"top": None} if case["top"] else {})
+
+
+def exact(case, seed):
+    if case["op"] == "copy":
+        return None
+    s = prepare(case, seed)
+    return _exact_tree(case, s) if case["op"] == "tree" else _exact_append(case, s) if case["op"] == "append" else _exact_logprobs(case, s)
