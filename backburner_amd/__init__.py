@@ -23,6 +23,7 @@ LIB_SYNTH = PKG / "libpa_synth.so"
 
 FMT_F16, FMT_Q8_0, FMT_Q4_0 = 0, 1, 2          # config_req.is_q8 (phone-attn.h:15, 88)
 QMODE_GGML, QMODE_F16 = 0, 1
+TYPE_F32, TYPE_F16, TYPE_BF16 = 0, 1, 2          # activations and logits
 PAGE = 4096                                      # keys per page (phone-attn.h:160)
 
 
@@ -39,6 +40,13 @@ class Shape(C.Structure):
     """pa_hip_shape: nkv, rows per KV head, hd, fmt, rs, hb, qmode, scale."""
     _fields_ = [("nkv", C.c_uint32), ("rows", C.c_uint32), ("hd", C.c_uint32), ("fmt", C.c_uint32),
                 ("rs", C.c_uint32), ("hb", C.c_uint32), ("qmode", C.c_uint32), ("scale", C.c_float)]
+
+
+class Rope(C.Structure):
+    """pa_hip_rope: the norm weights, frequencies and layout of pa_hip_append_rope (make_rope)."""
+    _fields_ = [("q_weight", C.c_void_p), ("k_weight", C.c_void_p), ("inv_freq", C.c_void_p), ("eps", C.c_float),
+                ("n_rot", C.c_uint32), ("interleaved", C.c_uint32), ("type", C.c_uint32), ("q_stride", C.c_uint64),
+                ("k_stride", C.c_uint64), ("v_stride", C.c_uint64)]
 
 
 _hip = None
@@ -120,6 +128,18 @@ def lib() -> C.CDLL:
     L.pa_hip_append_f32.restype = C.c_int
     L.pa_hip_append_f32.argtypes = [C.POINTER(Shape), C.POINTER(vp), C.POINTER(vp), C.c_int, C.c_uint32, C.c_uint32, vp, vp,
                                     C.c_uint32, vp]
+    L.pa_hip_attn_tree.restype = C.c_int
+    L.pa_hip_attn_tree.argtypes = [vp, C.POINTER(Shape), C.POINTER(vp), C.POINTER(vp), C.POINTER(C.c_uint32), C.c_int, C.c_uint32, vp,
+                                   vp, vp, vp, vp]
+    L.pa_hip_logprobs.restype = C.c_int
+    L.pa_hip_logprobs.argtypes = [vp, vp, C.c_int, C.c_int, C.c_int64, C.c_int64, C.c_float, vp, C.c_int, C.c_int, vp, vp, vp, vp, vp,
+                                  vp]
+    L.pa_hip_append_rope.restype = C.c_int
+    L.pa_hip_append_rope.argtypes = [C.POINTER(Shape), C.POINTER(vp), C.POINTER(vp), C.c_int, C.c_uint32, C.c_uint32, C.POINTER(Rope),
+                                     vp, vp, vp, vp, C.c_uint32, vp, vp]
+    L.pa_hip_copy_rows.restype = C.c_int
+    L.pa_hip_copy_rows.argtypes = [C.POINTER(Shape), C.c_int, C.POINTER(vp), C.POINTER(vp), C.c_int, C.POINTER(vp), C.POINTER(vp),
+                                   C.c_int, C.c_uint32, C.POINTER(C.c_uint32), C.c_uint32, C.c_uint32, C.c_uint32, vp]
     L.pa_hip_coattn_merge.restype = C.c_int
     L.pa_hip_coattn_merge.argtypes = [vp, vp, vp, vp, vp, C.c_uint64, C.c_uint32, vp, vp, vp]
     _hip = L
@@ -313,6 +333,32 @@ class Pages:
             b.close()
 
 
+class PageTable:
+    """The page table of `pages` as a call takes it, built once for a loop of calls (pages changed later need a new one)."""
+
+    def __init__(self, pages: Pages):
+        self.n = len(pages.k)
+        m = max(self.n, 1)
+        self.k, self.v = (C.c_void_p * m)(*pages.k), (C.c_void_p * m)(*pages.v)
+        self.nkeys = (C.c_uint32 * m)(*pages.nkeys)
+
+
+def _table(pages) -> PageTable:
+    return pages if isinstance(pages, PageTable) else PageTable(pages)
+
+
+class LayerTable:
+    """The pages of several layers (a list of Pages, each with as many pages), as copy_rows takes them."""
+
+    def __init__(self, layers: list):
+        self.layers, self.pages = len(layers), len(layers[0].k) if layers else 0
+        if any(len(p.k) != self.pages or len(p.v) != self.pages for p in layers):
+            raise PaHipError("LayerTable: every layer needs the same number of pages")
+        m = max(self.layers * self.pages, 1)
+        self.k = (C.c_void_p * m)(*[x for p in layers for x in p.k])
+        self.v = (C.c_void_p * m)(*[x for p in layers for x in p.v])
+
+
 class Workspace:
     """pa_hip_ws: split-K partials and prepared Q of one stream."""
 
@@ -348,6 +394,20 @@ class Workspace:
     def time_next(self, ev_start, ev_end) -> None:
         """Record ev_start / ev_end around the attention kernel of the next attn() call."""
         _check(lib().pa_hip_ws_time_next(self.ptr, ev_start, ev_end), "pa_hip_ws_time_next")
+
+    def attn_tree(self, shape: Shape, pages, n_nodes: int, mask: int, Q: int, Oh: int, lse: int, stream=None) -> None:
+        """Enqueue pa_hip_attn_tree: the last n_nodes keys of `pages` (Pages or PageTable) are the drafted tree's, mask (device
+        uint64 [n_nodes]) says which of them each node sees; the reply format at Oh, lse."""
+        t = _table(pages)
+        _check(lib().pa_hip_attn_tree(self.ptr, C.byref(shape), t.k, t.v, t.nkeys, t.n, n_nodes, mask, Q, Oh, lse, stream),
+               "pa_hip_attn_tree")
+
+    def logprobs(self, logits: int, type: int, n_rows: int, vocab: int, row_stride: int, scale: float, given, n_given: int, n_top: int,
+                 logp, lse, entropy, top_id=None, top_logp=None, stream=None) -> None:
+        """Enqueue pa_hip_logprobs: log probabilities of given ids, log-sum-exp, entropy and the n_top best alternatives of each row
+        (device pointers)."""
+        _check(lib().pa_hip_logprobs(self.ptr, logits, type, n_rows, vocab, row_stride, scale, given, n_given, n_top, logp, lse, entropy,
+                                     top_id, top_logp, stream), "pa_hip_logprobs")
 
     def accept(self, logits: int, n_rows: int, vocab: int, draft: int, out: int, stream=None) -> None:
         _check(lib().pa_hip_accept(self.ptr, logits, n_rows, vocab, draft, out, stream), "pa_hip_accept")
@@ -408,6 +468,33 @@ def append_f32(shape: Shape, pages: Pages, page_keys: int, pos0: int, K: int, V:
     m = max(len(pages.k), 1)
     kp = (C.c_void_p * m)(*pages.k); vp = (C.c_void_p * m)(*pages.v)
     _check(lib().pa_hip_append_f32(C.byref(shape), kp, vp, len(pages.k), page_keys, pos0, K, V, n, stream), "pa_hip_append_f32")
+
+
+def make_rope(q_weight, k_weight, eps: float, inv_freq, n_rot: int, interleaved: bool = False, type: int = TYPE_F32,
+              q_stride: int = 0, k_stride: int = 0, v_stride: int = 0) -> Rope:
+    """pa_hip_rope of device pointers (weights None: no norm); strides in elements from token to token, 0 = packed."""
+    return Rope(q_weight, k_weight, inv_freq, eps, n_rot, int(interleaved), type, q_stride, k_stride, v_stride)
+
+
+def append_rope(shape: Shape, pages, page_keys: int, pos0: int, rope: Rope, Q, K: int, V: int, positions: int, n: int, q_out,
+                stream=None) -> None:
+    """pa_hip_append_rope: n tokens' queries and keys normed and rotated; queries to q_out, keys and values quantized into `pages`
+    (Pages or PageTable) at pos0. Q and q_out None: keys and values only."""
+    t = _table(pages)
+    _check(lib().pa_hip_append_rope(C.byref(shape), t.k, t.v, t.n, page_keys, pos0, C.byref(rope), Q, K, V, positions, n, q_out, stream),
+           "pa_hip_append_rope")
+
+
+def copy_rows(shape: Shape, src: LayerTable, dst: LayerTable, page_keys: int, src_pos, dst_pos0: int, stream=None) -> None:
+    """pa_hip_copy_rows: the rows at positions src_pos (increasing; a range for consecutive ones) of every layer to dst_pos0 ..;
+    src and dst may be the same table."""
+    if src.layers != dst.layers:
+        raise PaHipError("copy_rows: src and dst need the same number of layers")
+    n = len(src_pos)
+    one = isinstance(src_pos, range) and src_pos.step == 1
+    at = None if one else (C.c_uint32 * max(n, 1))(*src_pos)
+    _check(lib().pa_hip_copy_rows(C.byref(shape), src.layers, src.k, src.v, src.pages, dst.k, dst.v, dst.pages, page_keys, at,
+                                  src_pos.start if one and n else 0, dst_pos0, n, stream), "pa_hip_copy_rows")
 
 
 def alloc_pages(n_pages: int, page_bytes: int) -> Pages:

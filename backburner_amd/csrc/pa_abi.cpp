@@ -58,6 +58,8 @@ bool device_usable() {
     return true;
 }
 
+bool aligned(const void * p, uintptr_t a) { return ((uintptr_t) p & (a - 1)) == 0; }
+
 uint32_t head_bytes(int fmt, int hd) {
     return fmt == PA_FMT_Q8_0 ? (uint32_t) (hd / 32 * 34) : fmt == PA_FMT_Q4_0 ? (uint32_t) (hd / 32 * 18) : (uint32_t) (hd * 2);
 }
@@ -71,6 +73,9 @@ struct pa_hip_ws {
     float2 * pml = nullptr; size_t pml_cap = 0;
     unsigned long long * apart = nullptr; size_t apart_cap = 0;
     unsigned int * acount = nullptr;
+    // pa_hip_logprobs: a row's parts and their best keys
+    float4 * lpart = nullptr; size_t lpart_cap = 0;
+    unsigned long long * lkeys = nullptr; size_t lkeys_cap = 0;
     // buffers replaced by a larger one: a graph captured earlier may still name them, so they live as long as the
     // workspace (growth at least doubles a buffer, so they hold less than the live ones)
     std::vector<void *> retired;
@@ -147,7 +152,8 @@ extern "C" void pa_hip_ws_destroy(pa_hip_ws * w) {
     if (w->broken) return;   // a timed-out call may still be using its buffers: they are left to the process
     (void) hipDeviceSynchronize();
     for (void * p : {(void *) w->po, (void *) w->pml, (void *) w->apart, (void *) w->acount, (void *) w->dk,
-                     (void *) w->dv, (void *) w->dq, (void *) w->dout, (void *) w->ro, (void *) w->rml})
+                     (void *) w->dv, (void *) w->dq, (void *) w->dout, (void *) w->ro, (void *) w->rml, (void *) w->lpart,
+                     (void *) w->lkeys})
         (void) hipFree(p);
     for (void * p : w->retired) (void) hipFree(p);
     if (w->hst) (void) hipHostFree(w->hst);
@@ -224,6 +230,8 @@ struct Call {
     uint16_t * reply_oh = nullptr;
     float * reply_lse = nullptr;
     bool reply_done = false;
+    TreeArgs * tree = nullptr;        // pa_hip_attn_tree: the call's pages are its context, the merge joins the drafted keys
+    uint32_t fmt = 0;
     float * po = nullptr;
     float2 * pml = nullptr;
 
@@ -262,6 +270,12 @@ struct Call {
     }
     // the merge of the call's slots: the reply format when asked for, else (O, m, l)
     bool merge(MergeArgs & ma, int hd, hipStream_t st) {
+        if (tree) {
+            tree->m = ma;
+            tree->m.Oh = reply_oh; tree->m.lse = reply_lse;
+            reply_done = true;
+            return hip_ok(launch_tree(hd, (int) fmt, *tree, st), "tree launch");
+        }
         if (reply_oh) { ma.Oh = reply_oh; ma.lse = reply_lse; reply_done = true; }
         return hip_ok(launch_merge(hd, ma, st), "merge launch");
     }
@@ -335,7 +349,7 @@ int attn_decode(Call & cx, const pa_hip_shape * s, const void * const * k_pages,
         n_slots = 0;
         for_launches(nkeys, n_pages, [&](int, int, uint64_t tiles, uint64_t) { n_slots += groups(tiles, cap); });
     }
-    const bool direct = n_launch == 1 && n_slots == 1;
+    const bool direct = n_launch == 1 && n_slots == 1 && !cx.tree;
     if (!direct && !cx.slots(n_slots * rows_per_slot, s->hd, st)) return -1;
     uint32_t li = 0, slot0 = 0;
     bool ok = true;
@@ -354,7 +368,7 @@ int attn_decode(Call & cx, const pa_hip_shape * s, const void * const * k_pages,
         a.q = Q; a.po = cx.po; a.pml = cx.pml; a.O = O; a.m = m; a.l = l;
         const uint32_t grid = (a.n_items + 7) / 8 * 8;
         // the timing events (if any) at the start of the first and the end of the last decode kernel
-        ok = hip_ok(launch_decode((int) s->fmt, a, grid, st, li == 0 ? cx.ev0 : nullptr, li + 1 == n_launch ? cx.ev1 : nullptr),
+        ok = hip_ok(launch_decode((int) s->fmt, cx.tree != nullptr, a, grid, st, li == 0 ? cx.ev0 : nullptr, li + 1 == n_launch ? cx.ev1 : nullptr),
                     "decode launch");
         li++;
         slot0 += ng;
@@ -482,7 +496,7 @@ bool mma_wide256(const pa_hip_shape * s, const uint32_t * nkeys, int n_pages) {
 // the other head-dim-256 calls
 int attn_mma(Call & cx, const pa_hip_shape * s, const void * const * k_pages, const void * const * v_pages,
              const uint32_t * nkeys, int n_pages, const float * Q, float * O, float * m, float * l, hipStream_t st) {
-    const MmaForm form = mma_form(s, mma_wide256(s, nkeys, n_pages));
+    const MmaForm form = mma_form(s, !cx.tree && mma_wide256(s, nkeys, n_pages));
     const uint32_t nw = form.nw, rpw = form.rpw, nrb = form.nrb, units = form.units;
     const bool h256 = form.h256;
     // rows per KV head in the slots: whole row blocks, at head dim 256 multiples of 64 under either kernel (only real rows
@@ -520,7 +534,7 @@ int attn_mma(Call & cx, const pa_hip_shape * s, const void * const * k_pages, co
         n_slots = 0;
         for_launches(nkeys, n_pages, [&](int, int, uint64_t tiles, uint64_t) { n_slots += chunking(tiles, cap, tpc); });
     }
-    const bool direct = n_launch == 1 && n_slots == 1;
+    const bool direct = n_launch == 1 && n_slots == 1 && !cx.tree;
     // a workspace gets the room that one round of workgroups of either kernel would take over this context, whatever the
     // context pays for, so that calls of other shapes find what they need there when they are captured
     if (!cx.fixed && cx.mma_workgroups == 0 && cx.chunk_keys == 0) {
@@ -565,8 +579,8 @@ int attn_mma(Call & cx, const pa_hip_shape * s, const void * const * k_pages, co
         // 25.9), up to 32 rows, where a quarter of the waves still idles, from about 32 (48 tiles 58.7 / 56.2, 17 tiles 30.5
         // / 31.5)
         const int streams = s->hd == 128 && s->rows <= 64 && tpc >= (s->rows > 32 ? 10u : 32u) ? 2 : 1;
-        ok = hip_ok(h256 ? launch_mma256((int) s->fmt, skip, a, grid, st, e0, e1)
-                         : launch_mma((int) s->hd, (int) s->fmt, (int) nw, skip, streams, a, grid, st, e0, e1), "mma launch");
+        ok = hip_ok(h256 ? launch_mma256((int) s->fmt, skip, cx.tree != nullptr, a, grid, st, e0, e1)
+                         : launch_mma((int) s->hd, (int) s->fmt, (int) nw, skip, streams, cx.tree != nullptr, a, grid, st, e0, e1), "mma launch");
         li++;
         slot0 += nch;
     });
@@ -581,8 +595,8 @@ int attn_mma(Call & cx, const pa_hip_shape * s, const void * const * k_pages, co
 
 // the argument checks every engine-path attention call shares; false (with the message set) on a bad argument
 // (the message strings are built on the error path only: a good call allocates nothing on the host either)
-bool attn_args_ok(const char * fn, const pa_hip_shape * s, const void * const * k_pages, const void * const * v_pages,
-                  const uint32_t * nkeys, int n_pages, const float * Q, const float * O, const float * m, const float * l) {
+bool attn_pages_ok(const char * fn, const pa_hip_shape * s, const void * const * k_pages, const void * const * v_pages,
+                   const uint32_t * nkeys, int n_pages) {
     auto bad = [&](const std::string & why) { set_err(std::string(fn) + ": " + why); return false; };
     if (!s) return bad("null shape");
     if (s->hd != 128 && s->hd != 256) return bad("hd must be 128 or 256");
@@ -596,14 +610,20 @@ bool attn_args_ok(const char * fn, const pa_hip_shape * s, const void * const * 
     // a kernel's per-tile buffer range spans at most 32 rows of rs bytes in 32 bits
     if (s->rs >= (1u << 26)) return bad("rs must be below 2^26 bytes");
     if (n_pages < 0 || (n_pages > 0 && (!k_pages || !v_pages || !nkeys))) return bad("bad page table");
-    if (!Q || !O || !m || !l) return bad("null Q/O/m/l");
-    if (((uintptr_t) O & 15) || ((uintptr_t) Q & 3)) return bad("O must be 16-byte and Q 4-byte aligned");
     uint64_t total = 0;
     for (int i = 0; i < n_pages; i++) {
         if (nkeys[i] > 0 && (!k_pages[i] || !v_pages[i])) return bad("null page " + std::to_string(i));
         total += nkeys[i];
     }
     if (total > 0xffffffffull) return bad("more than 2^32 - 1 keys");
+    return true;
+}
+
+bool attn_args_ok(const char * fn, const pa_hip_shape * s, const void * const * k_pages, const void * const * v_pages,
+                  const uint32_t * nkeys, int n_pages, const float * Q, const float * O, const float * m, const float * l) {
+    if (!attn_pages_ok(fn, s, k_pages, v_pages, nkeys, n_pages)) return false;
+    if (!Q || !O || !m || !l) { set_err(std::string(fn) + ": null Q/O/m/l"); return false; }
+    if (((uintptr_t) O & 15) || ((uintptr_t) Q & 3)) { set_err(std::string(fn) + ": O must be 16-byte and Q 4-byte aligned"); return false; }
     return true;
 }
 
@@ -740,7 +760,6 @@ bool rows_ok(const char * fn, uint64_t rows, uint32_t hd) {
     if (rows > (1ull << 24)) { set_err(std::string(fn) + ": more than 2^24 rows"); return false; }   // 2^22 workgroups
     return true;
 }
-bool aligned(const void * p, uintptr_t a) { return ((uintptr_t) p & (a - 1)) == 0; }
 }  // namespace
 
 extern "C" int pa_hip_merge_partial(float * O, float * m, float * l, const float * O2, const float * m2, const float * l2,
@@ -769,6 +788,75 @@ extern "C" int pa_hip_coattn_merge(const uint16_t * Oh, const float * lse, const
     }
     return hip_ok(launch_coattn((int) hd, Oh, lse, O_loc, m_loc, l_loc, rows, out, lse_out, (hipStream_t) stream),
                   "coattn launch") ? 0 : -1;
+}
+
+// The context goes through the attention kernels, whose slots (never a direct result) the tree kernel joins with the drafted
+// keys: their rows' addresses travel in its arguments, so they may lie in any pages.
+extern "C" int pa_hip_attn_tree(pa_hip_ws * ws, const pa_hip_shape * s, const void * const * k_pages, const void * const * v_pages,
+                                const uint32_t * nkeys, int n_pages, uint32_t n_nodes, const uint64_t * mask, const float * Q,
+                                uint16_t * Oh, float * lse, void * stream) {
+    const char * fn = "pa_hip_attn_tree";
+    auto bad = [&](const std::string & why) { set_err(std::string(fn) + ": " + why); return -1; };
+    if (!attn_pages_ok(fn, s, k_pages, v_pages, nkeys, n_pages)) return -1;
+    if (n_nodes < 1 || n_nodes > 64) return bad("n_nodes must be 1..64");
+    if (s->rows % n_nodes) return bad("rows must be a multiple of n_nodes");
+    if (s->qmode != PA_QMODE_GGML) return bad("qmode must be 0 (ggml)");
+    if ((uint64_t) s->nkv * s->rows > (1ull << 24)) return bad("more than 2^24 rows");
+    if (!mask || !Q || !Oh || !lse) return bad("null mask/Q/Oh/lse");
+    if (!aligned(mask, 8) || !aligned(Q, 4) || !aligned(Oh, 8) || !aligned(lse, 4))
+        return bad("mask and Oh must be 8-byte, Q and lse 4-byte aligned");
+    // the last n_nodes keys, from the last page back; what is left is the context
+    static thread_local std::vector<uint32_t> context;
+    context.assign(nkeys, nkeys + n_pages);
+    TreeArgs ta;
+    std::memset(&ta, 0, sizeof ta);
+    uint32_t left = n_nodes;
+    for (int p = n_pages - 1; p >= 0 && left > 0; p--)
+        while (context[p] > 0 && left > 0) {
+            const size_t off = (size_t) --context[p] * s->rs;
+            left--;
+            ta.k[left] = (const uint8_t *) k_pages[p] + off;
+            ta.v[left] = (const uint8_t *) v_pages[p] + off;
+        }
+    if (left > 0) return bad("fewer keys than n_nodes");
+    if (!ws) return bad("null workspace");
+    ta.mask = mask; ta.q = Q; ta.n_nodes = n_nodes; ta.hb = s->hb; ta.scale = s->scale;
+    Call cx;
+    cx.ws = ws;
+    cx.dec_groups = ws->dec_groups; cx.mma_workgroups = ws->mma_workgroups; cx.chunk_keys = ws->chunk_keys;
+    cx.ev0 = ws->ev0; cx.ev1 = ws->ev1;
+    ws->ev0 = ws->ev1 = nullptr;
+    cx.reply_oh = Oh; cx.reply_lse = lse; cx.tree = &ta; cx.fmt = s->fmt;
+    return attn_call(cx, s, k_pages, v_pages, context.data(), n_pages, Q, nullptr, nullptr, nullptr, (hipStream_t) stream);
+}
+
+extern "C" int pa_hip_logprobs(pa_hip_ws * ws, const void * logits, int type, int n_rows, int64_t vocab, int64_t row_stride, float scale,
+                               const int32_t * given, int n_given, int n_top, float * logp, float * lse, float * entropy,
+                               int32_t * top_id, float * top_logp, void * stream) {
+    auto bad = [&](const char * why) { set_err(std::string("pa_hip_logprobs: ") + why); return -1; };
+    if (type < PA_TYPE_F32 || type > PA_TYPE_BF16) return bad("type must be 0 (f32), 1 (f16) or 2 (bf16)");
+    if (n_rows < 0 || n_rows > (1 << 20)) return bad("n_rows must be 0..2^20");
+    if (vocab < 1 || vocab > (1 << 24)) return bad("vocab must be 1..2^24");
+    if (row_stride < vocab || row_stride > (1ll << 40)) return bad("row_stride must be vocab..2^40");
+    if (!(scale > 0.0f) || !std::isfinite(scale)) return bad("scale must be finite and > 0");
+    if (n_given < 0 || n_given > 1024 || n_top < 0 || n_top > 32) return bad("n_given must be 0..1024 and n_top 0..32");
+    if (n_rows == 0) return 0;
+    if (!logits || (n_given > 0 && (!given || !logp)) || (n_top > 0 && (!top_id || !top_logp))) return bad("null argument");
+    if (!aligned(logits, type == PA_TYPE_F32 ? 4 : 2) || !aligned(given, 4) || !aligned(logp, 4) || !aligned(lse, 4) || !aligned(entropy, 4) ||
+        !aligned(top_id, 4) || !aligned(top_logp, 4))
+        return bad("logits must be aligned to their type, the other arrays to 4 bytes");
+    if (!ws) return bad("null workspace");
+    LogprobArgs a;
+    a.seg = (int64_t) n_rows * ((vocab + 4095) / 4096) <= 1024 ? 4096 : 16384;
+    a.splits = (int) ((vocab + a.seg - 1) / a.seg);
+    hipStream_t st = (hipStream_t) stream;
+    const size_t parts = (size_t) n_rows * a.splits;
+    if (!ensure(ws, ws->lpart, ws->lpart_cap, parts * sizeof(float4), st, true, "hipMalloc logprob parts")) return -1;
+    if (n_top > 0 && !ensure(ws, ws->lkeys, ws->lkeys_cap, parts * n_top * sizeof(unsigned long long), st, true, "hipMalloc logprob keys")) return -1;
+    a.logits = logits; a.given = given; a.logp = logp; a.lse = lse; a.entropy = entropy; a.top_logp = top_logp; a.top_id = top_id;
+    a.part = ws->lpart; a.keys = ws->lkeys; a.vocab = vocab; a.stride = row_stride; a.scale = scale; a.type = type;
+    a.n_rows = n_rows; a.n_given = n_given; a.n_top = n_top;
+    return hip_ok(launch_logprobs(a, st), "logprobs launch") ? 0 : -1;
 }
 
 // ---------------------------------------------------------------- 4. KV ingest into HBM pages
@@ -804,26 +892,36 @@ bool pages_aligned(const char * fn, void * const * kp, void * const * vp, uint32
     return true;
 }
 
-// the launches of a converting APPEND: rows of up to APPEND_SEGS pages each, at most 65,535 (a grid dimension) and 2^23 workgroups;
-// `row` = bytes of a source row, the rest of `a` filled in
-int append_launches(AppendArgs & a, bool from_f32, void * const * kp, void * const * vp, uint32_t page_keys, uint32_t pos0,
-                    const uint8_t * K, const uint8_t * V, size_t row, uint32_t n, hipStream_t st) {
-    const uint64_t max_rows = std::min<uint64_t>(65535, std::max<uint64_t>(1, (1u << 23) / ((2ull * a.nkv * (a.hd / 32) + 15) / 16)));
+// the launches of a converting APPEND: rows of up to APPEND_SEGS pages each, at most 65,535 (a grid dimension) and 2^23 workgroups
+// of wpr per row; launch(first row) enqueues one, with the page fields of `a` filled in
+template <class F>
+int append_launches(AppendArgs & a, uint64_t wpr, void * const * kp, void * const * vp, uint32_t page_keys, uint32_t pos0, uint32_t n,
+                    const char * what, F launch) {
+    const uint64_t max_rows = std::min<uint64_t>(65535, std::max<uint64_t>(1, (1u << 23) / wpr));
     for (uint32_t done = 0; done < n;) {
         const uint32_t pi = (pos0 + done) / page_keys, off = (pos0 + done) % page_keys;
         const uint32_t take = (uint32_t) std::min<uint64_t>({n - done, max_rows, (uint64_t) APPEND_SEGS * page_keys - off});
         a.off0 = off; a.page_keys = page_keys; a.n = take;
-        a.ksrc = K + (size_t) done * row;
-        a.vsrc = V + (size_t) done * row;
         const uint32_t last = (uint32_t) (((uint64_t) off + take - 1) / page_keys);
         for (uint32_t i = 0; i < (uint32_t) APPEND_SEGS; i++) {
             a.kdst[i] = i <= last ? (uint8_t *) kp[pi + i] : nullptr;
             a.vdst[i] = i <= last ? (uint8_t *) vp[pi + i] : nullptr;
         }
-        if (!hip_ok(launch_append(from_f32, a, st), from_f32 ? "append quantize launch" : "append f16 launch")) return -1;
+        if (!hip_ok(launch(done), what)) return -1;
         done += take;
     }
     return 0;
+}
+
+// ... of rows that come one after the other: `row` = bytes of a source row, the rest of `a` filled in
+int append_launches(AppendArgs & a, bool from_f32, void * const * kp, void * const * vp, uint32_t page_keys, uint32_t pos0,
+                    const uint8_t * K, const uint8_t * V, size_t row, uint32_t n, hipStream_t st) {
+    return append_launches(a, (2ull * a.nkv * (a.hd / 32) + 15) / 16, kp, vp, page_keys, pos0, n,
+                           from_f32 ? "append quantize launch" : "append f16 launch", [&](uint32_t done) {
+        a.ksrc = K + (size_t) done * row;
+        a.vsrc = V + (size_t) done * row;
+        return launch_append(from_f32, a, st);
+    });
 }
 }  // namespace
 
@@ -870,6 +968,132 @@ extern "C" int pa_hip_append_f32(const pa_hip_shape * s, void * const * k_pages,
     a.fmt = (int) s->fmt;
     return append_launches(a, true, k_pages, v_pages, page_keys, pos0, (const uint8_t *) K, (const uint8_t *) V,
                            (size_t) s->nkv * s->hd * sizeof(float), n, (hipStream_t) stream);
+}
+
+extern "C" int pa_hip_append_rope(const pa_hip_shape * s, void * const * k_pages, void * const * v_pages, int n_pages,
+                                  uint32_t page_keys, uint32_t pos0, const pa_hip_rope * rope, const void * Q, const void * K,
+                                  const void * V, const int32_t * positions, uint32_t n, float * q_out, void * stream) {
+    const char * fn = "pa_hip_append_rope";
+    auto bad = [&](const std::string & why) { set_err(std::string(fn) + ": " + why); return -1; };
+    if (!append_ok(fn, s, k_pages, v_pages, n_pages, page_keys, pos0, n)) return -1;
+    if (!rope) return bad("null rope");
+    if (rope->type > PA_TYPE_BF16) return bad("type must be 0 (f32), 1 (f16) or 2 (bf16)");
+    if (rope->n_rot > s->hd || rope->n_rot % 2) return bad("n_rot must be even and at most hd");
+    if (rope->n_rot > 0 && !rope->inv_freq) return bad("null inv_freq");
+    if (!(rope->eps >= 0.0f) || !std::isfinite(rope->eps)) return bad("eps must be finite and >= 0");
+    if (n == 0) return 0;
+    if (!K || !V || (rope->n_rot > 0 && !positions)) return bad("null K/V/positions");
+    if (!Q != !q_out) return bad("Q and q_out come together");
+    if (Q && (s->rows == 0 || s->rows % n)) return bad("rows must be a multiple of n");
+    const uint32_t gqa = Q ? s->rows / n : 0;
+    if ((uint64_t) s->nkv * (gqa + 2ull) > (1u << 20)) return bad("more than 2^20 heads");
+    RopeArgs r;
+    std::memset(&r, 0, sizeof r);
+    r.qst = rope->q_stride ? rope->q_stride : (uint64_t) s->nkv * gqa * s->hd;
+    r.kst = rope->k_stride ? rope->k_stride : (uint64_t) s->nkv * s->hd;
+    r.vst = rope->v_stride ? rope->v_stride : (uint64_t) s->nkv * s->hd;
+    if (r.qst > (1ull << 32) || r.kst > (1ull << 32) || r.vst > (1ull << 32)) return bad("strides must be at most 2^32");
+    if (rope->type != PA_TYPE_F32 && ((r.qst | r.kst | r.vst) & 1)) return bad("strides must be even for 16-bit types");
+    if (!aligned(Q, 4) || !aligned(K, 4) || !aligned(V, 4) || !aligned(positions, 4) || !aligned(q_out, 8) || !aligned(rope->inv_freq, 4) ||
+        !aligned(rope->q_weight, 4) || !aligned(rope->k_weight, 4))
+        return bad("q_out must be 8-byte, the other arrays 4-byte aligned");
+    const uint32_t al = s->fmt == PA_FMT_F16 ? 4 : 2;                // the stores are 32-bit (f16) or 16-bit words
+    if (s->rs % al || s->hb % al) return bad("rs and hb must be multiples of " + std::to_string(al));
+    if (!pages_aligned(fn, k_pages, v_pages, page_keys, pos0, n, al)) return -1;
+    r.a.nkv = s->nkv; r.a.hd = s->hd; r.a.rs = s->rs; r.a.hb = s->hb; r.a.fmt = (int) s->fmt;
+    r.q = Q; r.k = K; r.v = V; r.qw = rope->q_weight; r.kw = rope->k_weight; r.freq = rope->inv_freq; r.pos = positions; r.qout = q_out;
+    r.n = n; r.gqa = gqa; r.n_rot = rope->n_rot; r.interleaved = rope->interleaved != 0; r.type = (int) rope->type; r.eps = rope->eps;
+    return append_launches(r.a, s->nkv * (gqa + 2ull), k_pages, v_pages, page_keys, pos0, n, "append rope launch", [&](uint32_t done) {
+        r.t0 = done;
+        return launch_rope(r, (hipStream_t) stream);
+    });
+}
+
+// One launch covers up to COPY_SEGS (layer, tensor) pairs and rows of one source and one destination page: consecutive rows
+// between disjoint places in one (bulk), otherwise up to COPY_ROWS listed ones, in order, so that rows moved in place arrive as they were.
+extern "C" int pa_hip_copy_rows(const pa_hip_shape * s, int n_layers, const void * const * src_k, const void * const * src_v,
+                                int src_pages, void * const * dst_k, void * const * dst_v, int dst_pages, uint32_t page_keys,
+                                const uint32_t * src_pos, uint32_t src_pos0, uint32_t dst_pos0, uint32_t n, void * stream) {
+    auto bad = [&](const std::string & why) { set_err("pa_hip_copy_rows: " + why); return -1; };
+    if (!s || s->nkv == 0 || s->hb == 0 || (uint64_t) s->rs < (uint64_t) s->nkv * s->hb) return bad("bad shape");
+    if (s->rs >= (1u << 26)) return bad("rs must be below 2^26 bytes");
+    if (n_layers < 0 || src_pages < 0 || dst_pages < 0 || page_keys == 0) return bad("bad layer or page count");
+    if (n == 0 || n_layers == 0) return 0;
+    if (!src_k || !src_v || !dst_k || !dst_v) return bad("null page table");
+    bool consecutive = true;
+    if (src_pos)
+        for (uint32_t i = 1; i < n; i++) {
+            if (src_pos[i] <= src_pos[i - 1]) return bad("src_pos must be strictly increasing");
+            consecutive &= src_pos[i] == src_pos[i - 1] + 1;
+        }
+    const uint64_t first = src_pos ? src_pos[0] : src_pos0, last = src_pos ? src_pos[n - 1] : (uint64_t) src_pos0 + n - 1;
+    if (last >= (uint64_t) src_pages * page_keys) return bad("source positions past the last page");
+    const uint64_t dlast = (uint64_t) dst_pos0 + n - 1;
+    if (dlast >= (uint64_t) dst_pages * page_keys) return bad("destination positions past the last page");
+    const uint32_t sp0 = (uint32_t) (first / page_keys), sp1 = (uint32_t) (last / page_keys);
+    const uint32_t dp0 = dst_pos0 / page_keys, dp1 = (uint32_t) (dlast / page_keys);
+    // every touched page, to see which are both: (pointer, place of the table), destinations first
+    bool in_place = false;
+    {
+        static thread_local std::vector<std::pair<uintptr_t, uint64_t>> dst;
+        dst.clear();
+        auto place = [&](int layer, int tensor, uint32_t p) { return ((uint64_t) layer * 2 + tensor) << 32 | p; };
+        for (int l = 0; l < n_layers; l++)
+            for (int t = 0; t < 2; t++)
+                for (uint32_t p = dp0; p <= dp1; p++) {
+                    const void * x = (t ? dst_v : dst_k)[(size_t) l * dst_pages + p];
+                    if (!x) return bad("null destination page " + std::to_string(p) + " of layer " + std::to_string(l));
+                    dst.push_back({(uintptr_t) x, place(l, t, p)});
+                }
+        std::sort(dst.begin(), dst.end());
+        for (size_t i = 1; i < dst.size(); i++)
+            if (dst[i].first == dst[i - 1].first) return bad("a page is a destination twice");
+        for (int l = 0; l < n_layers; l++)
+            for (int t = 0; t < 2; t++)
+                for (uint32_t p = sp0; p <= sp1; p++) {
+                    const void * x = (t ? src_v : src_k)[(size_t) l * src_pages + p];
+                    if (!x) return bad("null source page " + std::to_string(p) + " of layer " + std::to_string(l));
+                    const auto at = std::lower_bound(dst.begin(), dst.end(), std::make_pair((uintptr_t) x, (uint64_t) 0));
+                    if (at == dst.end() || at->first != (uintptr_t) x) continue;
+                    if (at->second != place(l, t, p)) return bad("a page is a source and, at another place, a destination");
+                    in_place = true;
+                }
+    }
+    auto from = [&](uint32_t i) { return src_pos ? src_pos[i] : src_pos0 + i; };
+    // in place positions only move down (they ascend, so the first says so for all)
+    if (in_place && first < dst_pos0) return bad("rows moved in place must come from at or behind their destination");
+    uint32_t i0 = 0;
+    if (in_place) while (i0 < n && from(i0) == dst_pos0 + i0) i0++;  // rows that stay
+    const bool bulk = consecutive && (!in_place || first >= (uint64_t) dst_pos0 + n);
+    CopyArgs a;
+    a.rs = s->rs; a.row = s->nkv * s->hb;
+    while (i0 < n) {
+        const uint32_t sp = from(i0) / page_keys, dp = (dst_pos0 + i0) / page_keys;
+        a.from0 = from(i0) % page_keys; a.to0 = (dst_pos0 + i0) % page_keys;
+        uint32_t take = std::min(n - i0, page_keys - a.to0);
+        if (bulk) {
+            take = std::min(take, page_keys - a.from0);
+            // a launch's workgroups in 31 bits at any word size
+            take = std::min<uint64_t>(take, std::max<uint64_t>(1, (1ull << 40) / a.row));
+        } else {
+            take = std::min<uint32_t>(take, COPY_ROWS);
+            uint32_t k = 0;
+            while (k < take && from(i0 + k) / page_keys == sp) { a.from[k] = from(i0 + k) % page_keys; k++; }
+            take = k;
+        }
+        a.n = take;
+        for (int g0 = 0; g0 < 2 * n_layers; g0 += COPY_SEGS) {
+            a.segs = (uint32_t) std::min(COPY_SEGS, 2 * n_layers - g0);
+            for (uint32_t g = 0; g < a.segs; g++) {
+                const int l = (g0 + (int) g) / 2;
+                a.src[g] = (const uint8_t *) ((g & 1) ? src_v : src_k)[(size_t) l * src_pages + sp];
+                a.dst[g] = (uint8_t *) ((g & 1) ? dst_v : dst_k)[(size_t) l * dst_pages + dp];
+            }
+            if (!hip_ok(launch_copy(!bulk, a, (hipStream_t) stream), "copy launch")) return -1;
+        }
+        i0 += take;
+    }
+    return 0;
 }
 
 extern "C" int pa_hip_quantize(int fmt, const float * x, void * y, int64_t n, void * stream) {

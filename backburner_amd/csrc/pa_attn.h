@@ -49,12 +49,26 @@ struct MergeArgs {
     float * lse = nullptr;          // and lse = m + log l [nkv][rows] (0 and -inf where l = 0)
 };
 
+// pa_hip_attn_tree: the join of the prefix's split-K slots (`m`; n_slots 0: no prefix) with the draft's own keys, in the
+// reply format
+struct TreeArgs {
+    MergeArgs m;
+    const uint8_t * k[64], * v[64]; // key and value rows (head 0) of node j
+    const uint64_t * mask;          // [n_nodes]
+    const float * q;                // [nkv][rows][hd]
+    uint32_t n_nodes, hb;
+    float scale;
+};
+hipError_t launch_tree(int hd, int fmt, const TreeArgs & a, hipStream_t st);
+
 hipError_t launch_merge(int hd, const MergeArgs & a, hipStream_t st);
-hipError_t launch_decode(int fmt, const AttnArgs & a, uint32_t grid, hipStream_t st, hipEvent_t ev0 = nullptr,
+// px: probabilities kept to more bits than one fp16 rounding (ggml's query rounding at the 16-row and 32-row kernels' head dims only;
+// see the kernels)
+hipError_t launch_decode(int fmt, bool px, const AttnArgs & a, uint32_t grid, hipStream_t st, hipEvent_t ev0 = nullptr,
                          hipEvent_t ev1 = nullptr);
-hipError_t launch_mma(int hd, int fmt, int nw, bool skip, int streams, const AttnArgs & a, uint32_t grid, hipStream_t st, hipEvent_t ev0 = nullptr,
-                      hipEvent_t ev1 = nullptr);
-hipError_t launch_mma256(int fmt, bool skip, const AttnArgs & a, uint32_t grid, hipStream_t st, hipEvent_t ev0 = nullptr,
+hipError_t launch_mma(int hd, int fmt, int nw, bool skip, int streams, bool px, const AttnArgs & a, uint32_t grid, hipStream_t st,
+                      hipEvent_t ev0 = nullptr, hipEvent_t ev1 = nullptr);
+hipError_t launch_mma256(int fmt, bool skip, bool px, const AttnArgs & a, uint32_t grid, hipStream_t st, hipEvent_t ev0 = nullptr,
                          hipEvent_t ev1 = nullptr);
 hipError_t launch_quantize(int fmt, const float * x, void * y, int64_t n, hipStream_t st);
 
@@ -69,6 +83,30 @@ struct AppendArgs {                 // up to APPEND_SEGS page segments of an APP
     int fmt;                        // stored format (append_quant_kernel)
 };
 hipError_t launch_append(bool from_f32, const AppendArgs & a, hipStream_t st);
+
+struct RopeArgs {                   // pa_hip_append_rope: rows j = 0 .. a.n-1 of the launch are tokens t0 + j of the call
+    AppendArgs a;                   // pages, shape and fmt (ksrc, vsrc unused)
+    const void * q, * k, * v;       // token 0 of the call
+    const float * qw, * kw, * freq;
+    const int32_t * pos;
+    float * qout;                   // [nkv][gqa * n][hd]
+    uint64_t qst, kst, vst;         // elements from token to token
+    uint32_t t0, n, gqa, n_rot, interleaved;
+    int type;
+    float eps;
+};
+hipError_t launch_rope(const RopeArgs & a, hipStream_t st);
+
+constexpr int COPY_SEGS = 128;      // (layer, K or V) pairs of one copy launch
+constexpr int COPY_ROWS = 64;       // rows of a launch that takes a list of them
+struct CopyArgs {
+    const uint8_t * src[COPY_SEGS];
+    uint8_t * dst[COPY_SEGS];
+    uint32_t from[COPY_ROWS];       // rows of the source page (list form)
+    uint32_t from0, to0, n;         // first source row (bulk form), first destination row, rows
+    uint32_t segs, row, rs;         // bytes of a row, and from row to row
+};
+hipError_t launch_copy(bool list, const CopyArgs & a, hipStream_t st);
 hipError_t launch_merge_partial(int hd, float * O, float * m, float * l, const float * O2, const float * m2, const float * l2,
                                 uint64_t rows, hipStream_t st);
 hipError_t launch_normalise(int hd, const float * O, const float * m, const float * l, uint64_t rows, uint16_t * Oh,
@@ -87,6 +125,19 @@ struct AcceptArgs {
     int seg, segs;
 };
 hipError_t launch_accept(const AcceptArgs & a, hipStream_t st);
+
+struct LogprobArgs {
+    const void * logits;
+    const int32_t * given;
+    float * logp, * lse, * entropy, * top_logp;
+    int32_t * top_id;
+    float4 * part;                  // [n_rows][splits] (max, sum, weighted sum, NaN seen) of a workgroup's part of a row
+    unsigned long long * keys;      // [n_rows][splits][n_top] its best keys (orderable value, ~index), 0 where it has none
+    int64_t vocab, stride;
+    float scale;
+    int type, n_rows, n_given, n_top, splits, seg;   // seg: values per workgroup
+};
+hipError_t launch_logprobs(const LogprobArgs & a, hipStream_t st);
 
 // host side (pa_abi.cpp): the calling thread's last error, and the engine-path call with its split-K slots in a fixed
 // device array of `cap` bytes instead of a workspace (nothing allocated; the split adapts so the slots fit, and a call

@@ -1,0 +1,73 @@
+// pa_copy.hip - cache rows copied within and between pages, every layer's K and V in one launch (gfx950): the accepted path of a
+// draft tree moved together in place, and a fork's own copy of a page (pa_hip_copy_rows). No counterpart in the reference.
+//
+// copy_list_kernel   up to COPY_ROWS listed rows of one page, in place if asked: a thread owns a column of every row and takes
+//                    the rows in order, the loads of eight before their stores. In place row i comes from at or behind row to0 + i
+//                    and sources ascend, so a store never overwrites a row that a later batch still reads, and no other thread
+//                    touches the column.
+// copy_bulk_kernel   consecutive rows between disjoint places: four words per thread, their loads issued together.
+#include "pa_attn.h"
+#include "pa_common.h"
+
+namespace pa_hip {
+
+template <typename W> __global__ __launch_bounds__(256) void copy_list_kernel(const CopyArgs a) {
+    const uint32_t col = (blockIdx.x * 256 + threadIdx.x) * (uint32_t) sizeof(W);
+    if (col >= a.row) return;
+    const uint8_t * s = a.src[blockIdx.y] + col;
+    uint8_t * d = a.dst[blockIdx.y] + (size_t) a.to0 * a.rs + col;   // (may be the same page: no restrict)
+    for (uint32_t i = 0; i < a.n; i += 8) {
+        W x[8];
+        #pragma unroll
+        for (int u = 0; u < 8; u++)
+            if (i + u < a.n) x[u] = *(const W *) (s + (size_t) a.from[i + u] * a.rs);
+        #pragma unroll
+        for (int u = 0; u < 8; u++)
+            if (i + u < a.n) *(W *) (d + (size_t) (i + u) * a.rs) = x[u];
+    }
+}
+
+// per segment `words` words of type W; words per row wpr, 0 where rows follow each other without a gap
+template <typename W> __global__ __launch_bounds__(256) void copy_bulk_kernel(const CopyArgs a, uint64_t words, uint32_t wpr) {
+    const uint8_t * s = a.src[blockIdx.y] + (size_t) a.from0 * a.rs;
+    uint8_t * d = a.dst[blockIdx.y] + (size_t) a.to0 * a.rs;
+    const uint64_t w0 = (uint64_t) blockIdx.x * 1024 + threadIdx.x;
+    W x[4];
+    size_t at[4];
+    #pragma unroll
+    for (int u = 0; u < 4; u++) {
+        const uint64_t w = w0 + 256 * u;
+        at[u] = wpr == 0 ? w * sizeof(W) : (w / wpr) * a.rs + (w % wpr) * sizeof(W);
+        if (w < words) x[u] = *(const W *) (s + at[u]);
+    }
+    #pragma unroll
+    for (int u = 0; u < 4; u++)
+        if (w0 + 256 * u < words) *(W *) (d + at[u]) = x[u];
+}
+
+template <typename W> static hipError_t launch_copy_w(bool list, const CopyArgs & a, hipStream_t st) {
+    if (list) {
+        const uint32_t cols = a.row / sizeof(W);
+        hipLaunchKernelGGL(copy_list_kernel<W>, dim3((cols + 255) / 256, a.segs), dim3(256), 0, st, a);
+    } else {
+        const uint64_t words = (uint64_t) a.n * (a.row / sizeof(W));
+        const uint32_t wpr = a.row / sizeof(W);
+        const bool run = a.row == a.rs;
+        // (the host's checks keep a launch's words below 2^31 * 1024)
+        hipLaunchKernelGGL(copy_bulk_kernel<W>, dim3((uint32_t) ((words + 1023) / 1024), a.segs), dim3(256), 0, st, a, words,
+                           run ? (uint32_t) 0 : wpr);
+    }
+    return hipGetLastError();
+}
+
+hipError_t launch_copy(bool list, const CopyArgs & a, hipStream_t st) {
+    if (a.n == 0 || a.segs == 0) return hipSuccess;
+    uintptr_t al = a.row | a.rs;                                     // the widest word that every row starts and ends on
+    for (uint32_t i = 0; i < a.segs; i++) al |= (uintptr_t) a.src[i] | (uintptr_t) a.dst[i];
+    if (al % 16 == 0) return launch_copy_w<pa_u4>(list, a, st);
+    if (al % 4 == 0) return launch_copy_w<uint32_t>(list, a, st);
+    if (al % 2 == 0) return launch_copy_w<uint16_t>(list, a, st);
+    return launch_copy_w<uint8_t>(list, a, st);
+}
+
+}  // namespace pa_hip

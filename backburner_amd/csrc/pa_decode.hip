@@ -160,7 +160,8 @@ __device__ __forceinline__ void dec_lds_barrier() {
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
-template <int FMT>
+// PX: P' = P * d_v rounded to fp16 once (two roundings otherwise: P, then the product)
+template <int FMT, bool PX = false>
 __global__ __launch_bounds__(128, 2) void dec_kernel(const AttnArgs a) {
     using G = DecGeom<FMT>;
     constexpr int TCH = 32 * G::NCH;                                 // 16-byte chunks of one tensor's tile (544 / 288)
@@ -401,7 +402,14 @@ __global__ __launch_bounds__(128, 2) void dec_kernel(const AttnArgs a) {
         // ---- P' = P * d_v per V block -> LDS [block][key][row], then back transposed as the PV B operand
         #pragma unroll
         for (int b = 0; b < DEC_NKB; b++) {
-            const pa_u2 val = {pa_as_u32(p01 * dvh[b]), pa_as_u32(p23 * dvh[b])};
+            pa_u2 val;
+            if constexpr (PX) {
+                const float d = (float) dvh[b][0];
+                val = (pa_u2){pa_as_u32((pa_h2){(_Float16) (pr4[0] * d), (_Float16) (pr4[1] * d)}),
+                              pa_as_u32((pa_h2){(_Float16) (pr4[2] * d), (_Float16) (pr4[3] * d)})};
+            } else {
+                val = (pa_u2){pa_as_u32(p01 * dvh[b]), pa_as_u32(p23 * dvh[b])};
+            }
             *(pa_u2 *) (Pl + b * DEC_PBLK + kap * 16 + 8 * hh) = val;
         }
         dec_wave_sync();
@@ -475,9 +483,11 @@ __global__ __launch_bounds__(128, 2) void dec_kernel(const AttnArgs a) {
     }
 }
 
-hipError_t launch_decode(int fmt, const AttnArgs & a, uint32_t grid, hipStream_t st, hipEvent_t ev0, hipEvent_t ev1) {
+hipError_t launch_decode(int fmt, bool px, const AttnArgs & a, uint32_t grid, hipStream_t st, hipEvent_t ev0, hipEvent_t ev1) {
     // the events (optional) are recorded by the launch itself at the kernel's start and end
-    if (fmt == 1) hipExtLaunchKernelGGL((dec_kernel<1>), dim3(grid), dim3(128), 0, st, ev0, ev1, 0, a);
+    if (fmt == 1 && px) hipExtLaunchKernelGGL((dec_kernel<1, true>), dim3(grid), dim3(128), 0, st, ev0, ev1, 0, a);
+    else if (fmt == 2 && px) hipExtLaunchKernelGGL((dec_kernel<2, true>), dim3(grid), dim3(128), 0, st, ev0, ev1, 0, a);
+    else if (fmt == 1) hipExtLaunchKernelGGL((dec_kernel<1>), dim3(grid), dim3(128), 0, st, ev0, ev1, 0, a);
     else if (fmt == 2) hipExtLaunchKernelGGL((dec_kernel<2>), dim3(grid), dim3(128), 0, st, ev0, ev1, 0, a);
     else return hipErrorInvalidValue;
     return hipGetLastError();

@@ -3,6 +3,7 @@
 //   quantize_kernel        ggml quantize_row_q8_0_ref / quantize_row_q4_0_ref over contiguous 32-blocks
 //   append_quant_kernel    fp32 K/V rows [n][nkv][hd] quantized (or converted to f16) straight into page rows: the
 //                          sender's quantization of new keys, with no host round trip
+//   append_rope_kernel     the same from the model's projections: norm per head, position rotation, queries out
 //   append_f16_kernel      received q8_0 rows stored as f16 rows (the server's store_f16 mode, store_rows,
 //                          phone-attn.h:305-319)
 // The plain APPEND copy (phone-attn.h:403-421) is a device copy per page segment, issued by the host code.
@@ -120,6 +121,97 @@ __global__ __launch_bounds__(256) void append_quant_kernel(const AppendArgs a) {
     quant_block16(a.fmt, xb[2 * l], xb[2 * l + 1], l, t.row + (size_t) t.h * a.hb + (size_t) t.b * bb);
 }
 
+// ---------------------------------------------------------------- norm, rotation and append in one pass
+// Two consecutive values of a head as fp64 (exact for all three types)
+__device__ __forceinline__ void rope_load2(int type, const void * p, double & x0, double & x1) {
+    if (type == PA_TYPE_F32) {
+        const float2 v = *(const float2 *) p;
+        x0 = v.x; x1 = v.y;
+    } else {
+        const uint32_t u = *(const uint32_t *) p;
+        if (type == PA_TYPE_F16) {
+            x0 = pa_f16_bits_to_f32((uint16_t) u); x1 = pa_f16_bits_to_f32((uint16_t) (u >> 16));
+        } else {
+            x0 = __builtin_bit_cast(float, u << 16); x1 = __builtin_bit_cast(float, u & 0xffff0000u);
+        }
+    }
+}
+
+// Workgroup = one token and a share of its heads (queries, then keys, then values), a head per wave at a time: lane l holds dims
+// 2l, 2l + 1 (and 128 more of head dim 256), a quantizer's block then sits in 16 lanes.
+template <int HD>
+__global__ __launch_bounds__(256) void append_rope_kernel(const RopeArgs r) {
+    constexpr int NP = HD / 128;                                     // value pairs per lane
+    __shared__ double cs[HD / 2][2];                                 // cos, sin of the token's angles
+    __shared__ double ys[4][HD];                                     // a wave's normed head, for the pairs that span lanes
+    const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64;
+    const uint32_t j = blockIdx.y, t = r.t0 + j, half = r.n_rot / 2;
+    const uint32_t nq = r.q ? r.a.nkv * r.gqa : 0, nkv = r.a.nkv, heads = nq + 2 * nkv;
+    if ((uint32_t) tid < half) {
+        // the angle in turns: th = pos * f is exact (24 + 29 bits), 1 / (2 pi) in two parts, the whole turns taken out in between
+        const double th = (double) r.pos[t] * (double) r.freq[tid];
+        const double inv_hi = 0x1.45f306dc9c883p-3, inv_lo = -0x1.6b01ec5417056p-57;
+        const double whole = rint(th * inv_hi);
+        double c, s;
+        sincospi(2.0 * fma(th, inv_lo, fma(th, inv_hi, -whole)), &s, &c);
+        cs[tid][0] = c;
+        cs[tid][1] = s;
+    }
+    __syncthreads();
+    const uint32_t p = r.a.off0 + j, pg = p < r.a.page_keys ? 0u : p / r.a.page_keys;
+    const size_t prow = (size_t) (p - pg * r.a.page_keys) * r.a.rs;
+    for (uint32_t hj = blockIdx.x * 4 + wave; hj < heads; hj += gridDim.x * 4) {
+        const int kind = hj < nq ? 0 : hj < nq + nkv ? 1 : 2;        // query, key, value (uniform in the wave)
+        const uint32_t h = kind == 0 ? hj : kind == 1 ? hj - nq : hj - nq - nkv;
+        const size_t at = (size_t) t * (kind == 0 ? r.qst : kind == 1 ? r.kst : r.vst) + (size_t) h * HD + 2 * lane;
+        const uint8_t * src = (const uint8_t *) (kind == 0 ? r.q : kind == 1 ? r.k : r.v) + at * (r.type == PA_TYPE_F32 ? 4 : 2);
+        double y[2 * NP];
+        #pragma unroll
+        for (int i = 0; i < NP; i++) rope_load2(r.type, src + (size_t) i * 128 * (r.type == PA_TYPE_F32 ? 4 : 2), y[2 * i], y[2 * i + 1]);
+        if (kind < 2) {
+            const float * w = kind == 0 ? r.qw : r.kw;
+            if (w) {
+                double ss = 0;
+                #pragma unroll
+                for (int i = 0; i < 2 * NP; i++) ss += y[i] * y[i];
+                #pragma unroll
+                for (int off = 32; off > 0; off >>= 1) ss += __shfl_xor(ss, off);
+                const double f = 1.0 / sqrt(ss / HD + (double) r.eps);
+                #pragma unroll
+                for (int i = 0; i < 2 * NP; i++) y[i] *= f * (double) w[128 * (i / 2) + 2 * lane + (i & 1)];
+            }
+            if (half > 0) {
+                #pragma unroll
+                for (int i = 0; i < 2 * NP; i++) ys[wave][128 * (i / 2) + 2 * lane + (i & 1)] = y[i];
+                __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");   // one wave's LDS operations run in order
+                #pragma unroll
+                for (int i = 0; i < 2 * NP; i++) {
+                    const uint32_t d = 128 * (i / 2) + 2 * lane + (i & 1);
+                    if (d < r.n_rot) {
+                        const bool first = r.interleaved ? (d & 1) == 0 : d < half;
+                        const uint32_t f = r.interleaved ? d / 2 : first ? d : d - half;
+                        const double o = ys[wave][r.interleaved ? d ^ 1 : first ? d + half : d - half];
+                        y[i] = first ? y[i] * cs[f][0] - o * cs[f][1] : o * cs[f][1] + y[i] * cs[f][0];
+                    }
+                }
+                __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+            }
+        }
+        #pragma unroll
+        for (int i = 0; i < NP; i++) {
+            const float x0 = (float) y[2 * i], x1 = (float) y[2 * i + 1];
+            if (kind == 0) {
+                const size_t row = ((size_t) (h / r.gqa) * r.gqa + h % r.gqa) * r.n + t;
+                *(float2 *) (r.qout + row * HD + 128 * i + 2 * lane) = make_float2(x0, x1);
+            } else {
+                uint8_t * o = (kind == 1 ? r.a.kdst[pg] : r.a.vdst[pg]) + prow + (size_t) h * r.a.hb;
+                const uint32_t bb = r.a.fmt == 1 ? 34 : r.a.fmt == 2 ? 18 : 64;
+                quant_block16(r.a.fmt, x0, x1, lane % 16, o + (4 * i + lane / 16) * bb);
+            }
+        }
+    }
+}
+
 // received q8_0 block -> 32 f16 values f16(d * q) (d * q is exact in fp32, so the one rounding is the reference's);
 // lane l converts quants 2l, 2l+1
 __global__ __launch_bounds__(256) void append_f16_kernel(const AppendArgs a) {
@@ -147,6 +239,15 @@ hipError_t launch_append(bool from_f32, const AppendArgs & a, hipStream_t st) {
     const dim3 grid(wpr, a.n);                                       // n <= 65,535 (the host's launches)
     if (from_f32) hipLaunchKernelGGL(append_quant_kernel, grid, dim3(256), 0, st, a);
     else hipLaunchKernelGGL(append_f16_kernel, grid, dim3(256), 0, st, a);
+    return hipGetLastError();
+}
+
+hipError_t launch_rope(const RopeArgs & r, hipStream_t st) {
+    const uint32_t heads = (r.q ? r.a.nkv * r.gqa : 0) + 2 * r.a.nkv;
+    const dim3 grid((heads + 3) / 4, r.a.n);                         // n <= 65,535 (the host's launches)
+    if (r.a.hd == 128) hipLaunchKernelGGL(append_rope_kernel<128>, grid, dim3(256), 0, st, r);
+    else if (r.a.hd == 256) hipLaunchKernelGGL(append_rope_kernel<256>, grid, dim3(256), 0, st, r);
+    else return hipErrorInvalidValue;
     return hipGetLastError();
 }
 

@@ -76,7 +76,9 @@ __device__ __forceinline__ void mm_prep_q(const AttnArgs & a, uint32_t h, uint32
 // For q4_0 K (unsigned nibbles u = q + 8 in the int8 MFMA) it also gives, per block, the (hi, lo) pair of
 // -8 * (sum of the row's block quants) * (hi + lo) in fp32 (dcb[b]): the offset the unsigned nibbles add to each block
 // dot, times the row's scale pair; a key's block scale times it is that block's correction of the score.
-template <int HD, int FMT>
+// QS: the pair holds the factor times 2^QS, which keeps 22 bits down to 2^(-9-QS) (and takes factors up to 2^(16-QS)); the
+// integer dots are converted to 2^-QS of themselves for it.
+template <int HD, int FMT, int QS>
 __device__ __forceinline__ void mm_prep_qi8(const AttnArgs & a, uint32_t h, uint32_t row, bool rlive, int h2, pa_u4 (&Qi)[HD / 32],
                                             uint32_t (&dqb)[HD / 32], uint32_t (&dcb)[HD / 32]) {
     const float * qrow = a.q + ((size_t) h * a.rows + (rlive ? row : 0)) * HD + 16 * h2;
@@ -94,7 +96,8 @@ __device__ __forceinline__ void mm_prep_qi8(const AttnArgs & a, uint32_t h, uint
         am = mm_max32(am);                                           // the block's other 16 values: lane ^ 32
         const float d = am / 127.0f;
         const float id = d != 0.0f ? 1.0f / d : 0.0f;
-        const float dq = (float) (_Float16) d * (scale * MM_LOG2E);   // the fp16 block scale * scale, base-2 units
+        float dq = (float) (_Float16) d * (scale * MM_LOG2E);         // the fp16 block scale * scale, base-2 units
+        if constexpr (QS != 0) dq *= (float) (1 << QS);
         const _Float16 hi = (_Float16) dq, lo = (_Float16) (dq - (float) hi);
         if constexpr (HD == 256) dqb[b] = __builtin_bit_cast(uint32_t, dq * (FMT == 2 ? 0.0625f : 1.0f));
         else dqb[b] = (uint32_t) __builtin_bit_cast(uint16_t, hi) | ((uint32_t) __builtin_bit_cast(uint16_t, lo) << 16);
@@ -115,7 +118,8 @@ __device__ __forceinline__ void mm_prep_qi8(const AttnArgs & a, uint32_t h, uint
         if constexpr (FMT == 2 && HD == 128) {
             const auto t = __builtin_amdgcn_permlane32_swap((unsigned) qs, (unsigned) qs, false, false);
             const int qsum = (int) t[0] + (int) t[1];                // the block's 32 quants: lanes l and l ^ 32
-            const float c = (float) (-8 * qsum) * ((float) hi + (float) lo);
+            float c = (float) (-8 * qsum) * ((float) hi + (float) lo);
+            if constexpr (QS != 0) c *= 1.0f / (float) (1 << QS);
             const _Float16 chi = (_Float16) c, clo = (_Float16) (c - (float) chi);
             dcb[b] = (uint32_t) __builtin_bit_cast(uint16_t, chi) | ((uint32_t) __builtin_bit_cast(uint16_t, clo) << 16);
         }
@@ -170,11 +174,17 @@ __device__ __forceinline__ void mm_write_out(const AttnArgs & a, const mm_f16 (&
 // of every workgroup runs on SIMD i, half the SIMDs) only stage. The streams fold through LDS at the end, so the slots stay one
 // per workgroup. us per call with one stream and with two: 64 rows x 8 heads x 98,304 q4_0 keys 78.0 / 65.2, 40 rows x 33,333
 // q4_0 keys 36.8 / 34.0, 48 rows x 65,536 q4_0 keys (fp16 operands) 45.6 / 43.6.
-template <int HD, int FMT, int NW, bool SKIP, bool EX, int NS = 1>
+// PX: probabilities to more than one fp16 rounding, for results as exact as fp16 values allow: over quantized V, whose d*q is
+// rounded once, P enters as the fp16 pair (p, p - fp16(p)), two MFMAs instead of one; over f16 V, exact in fp16, as one; and
+// the row sum adds the fp32 probabilities. At head dim 128 the exact dots' scale pairs are held 2^6 times larger (QS in mm_prep_qi8:
+// the usual factors, fp16(d) / sqrt(128) of queries of size 1, lie at 2^-9, where lo falls into the subnormals and a score is off
+// by 1e-5, which a log-sum-exp shows).
+template <int HD, int FMT, int NW, bool SKIP, bool EX, int NS = 1, bool PX = false>
 __global__ __launch_bounds__(64 * NW, 8 / NW) void mma_kernel(const AttnArgs a) {   // 2 waves per SIMD
     static_assert(!EX || FMT != 0, "the exact block dots take quantized K");
     using G = MmGeom<HD>;
     constexpr int NBLK = G::NBLK;
+    constexpr int QS = PX && EX && HD == 128 ? 6 : 0;                // see mm_prep_qi8
     // tiles whose raw bytes are in flight in registers (head dim 256: one; O and Q take 192 of the 256 registers there, and
     // a tile's matrix work is twice as long)
     constexpr int PF = HD == 128 && NS == 1 ? 2 : 1;
@@ -307,7 +317,7 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void mma_kernel(const AttnArgs a) 
     uint32_t dqb[NBLK], dcb[NBLK];                                   // EX: the scale pairs; q4_0: the nibble-offset pairs
     #pragma unroll
     for (int b = 0; b < NBLK; b++) dqb[b] = dcb[b] = 0u;
-    if constexpr (EX) mm_prep_qi8<HD, FMT>(a, h, row, rlive, h2, Qi, dqb, dcb);
+    if constexpr (EX) mm_prep_qi8<HD, FMT, QS>(a, h, row, rlive, h2, Qi, dqb, dcb);
     else mm_prep_q<HD>(a, h, row, rlive, h2, Qf);
     // EX at head dim 128: the B operands of the scale products. All four products share one A operand, key n's block scales at k = 2b and
     // 2b + 1 (lanes h2 = b / 2, register b % 2), so block b's B operand holds row n's (hi, lo) pair there, zero elsewhere
@@ -329,7 +339,7 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void mma_kernel(const AttnArgs a) 
     // and SIMD with two waves)
     mm_i16 cvt0;
     #pragma unroll
-    for (int v = 0; v < 16; v++) cvt0[v] = 0x4B400000;
+    for (int v = 0; v < 16; v++) cvt0[v] = 0x4B400000 - (QS << 23);   // (QS: 2^-QS of it, 2^-QS dot)
     if constexpr (EX && HD == 128) asm volatile("" : "+v"(cvt0));         // kept in registers, not rebuilt for every tile
 
     // ---- prologue: tile t0 -> stage 0, tile t0 + 2's loads in flight in R0 (t0 + 1's in R1)
@@ -425,7 +435,7 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void mma_kernel(const AttnArgs a) 
                 const mm_f16 Pb = __builtin_amdgcn_mfma_f32_32x32x8f16(__builtin_bit_cast(pa_h4, dkw), __builtin_bit_cast(pa_h4, dqw[b]),
                                                                        (mm_f16){}, 0, 0, 0);
                 #pragma unroll
-                for (int v = 0; v < 16; v++) S[v] = fmaf(Pb[v], T[v] - 12582912.0f, b == 0 && FMT == 1 ? -mc : S[v]);
+                for (int v = 0; v < 16; v++) S[v] = fmaf(Pb[v], T[v] - 12582912.0f / (1 << QS), b == 0 && FMT == 1 ? -mc : S[v]);
                 __builtin_amdgcn_sched_barrier(0);
             }
             #pragma unroll
@@ -476,20 +486,33 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void mma_kernel(const AttnArgs a) 
             }
         }
         mx = fmaxf(mx, tm);
-        mm_h8 P[2];
-        #pragma unroll
-        for (int v = 0; v < 16; v++)
-            P[v / 8][v % 8] = (_Float16) __builtin_amdgcn_exp2f(EX ? S[v] : fmaf(S[v], sm, -mref));
-        #pragma unroll
-        for (int v = 0; v < 16; v += 2) {                            // the row sum of the fp16 P the PV MFMAs use
-            const mm_h2 pp = {P[v / 8][v % 8], P[v / 8][v % 8 + 1]};
-            lsum = __builtin_amdgcn_fdot2(pp, one2, lsum, false);
+        mm_h8 P[2], Pl[2];
+        if constexpr (PX) {
+            float ts[2] = {0.0f, 0.0f};
+            #pragma unroll
+            for (int v = 0; v < 16; v++) {
+                const float e = __builtin_amdgcn_exp2f(EX ? S[v] : fmaf(S[v], sm, -mref));
+                ts[v & 1] += e;
+                P[v / 8][v % 8] = (_Float16) e;
+                if constexpr (FMT != 0) Pl[v / 8][v % 8] = (_Float16) (e - (float) P[v / 8][v % 8]);
+            }
+            lsum += ts[0] + ts[1];
+        } else {
+            #pragma unroll
+            for (int v = 0; v < 16; v++)
+                P[v / 8][v % 8] = (_Float16) __builtin_amdgcn_exp2f(EX ? S[v] : fmaf(S[v], sm, -mref));
+            #pragma unroll
+            for (int v = 0; v < 16; v += 2) {                        // the row sum of the fp16 P the PV MFMAs use
+                const mm_h2 pp = {P[v / 8][v % 8], P[v / 8][v % 8 + 1]};
+                lsum = __builtin_amdgcn_fdot2(pp, one2, lsum, false);
+            }
         }
 
         // ---- O^T += V^T P^T
         #pragma unroll
         for (int i = 0; i < 2 * NBLK; i++) {
             O[i >> 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va[i % VA], P[i & 1], O[i >> 1], 0, 0, 0);
+            if constexpr (PX && FMT != 0) O[i >> 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va[i % VA], Pl[i & 1], O[i >> 1], 0, 0, 0);
             if (i + VA < 2 * NBLK) v_read(i + VA);
         }
     };
@@ -570,27 +593,34 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void mma_kernel(const AttnArgs a) 
 // The ggml query rounding over quantized K takes the exact block dots at every size (4-wave verify blocks and 8-wave
 // prefill chunks); the reference engines' rounding (PA_QMODE_F16) and f16 K take the fp16-operand QK, the Metal
 // engine's own arithmetic (K dequantized to half in threadgroup memory, pa-metal.mm:379-487)
-template <int HD, int FMT, bool EX>
+template <int HD, int FMT, bool EX, bool PX = false>
 static hipError_t launch_mma_fmt(int nw, bool skip, int streams, const AttnArgs & a, uint32_t grid, hipStream_t st, hipEvent_t ev0,
                                  hipEvent_t ev1) {
     switch (nw) {
         case 4:
-            if (streams == 2) hipExtLaunchKernelGGL((mma_kernel<128, FMT, 4, true, EX, 2>), dim3(grid), dim3(256), 0, st, ev0, ev1, 0, a);
-            else if (skip) hipExtLaunchKernelGGL((mma_kernel<HD, FMT, 4, true, EX>), dim3(grid), dim3(256), 0, st, ev0, ev1, 0, a);
-            else hipExtLaunchKernelGGL((mma_kernel<HD, FMT, 4, false, EX>), dim3(grid), dim3(256), 0, st, ev0, ev1, 0, a);
+            if (streams == 2) hipExtLaunchKernelGGL((mma_kernel<128, FMT, 4, true, EX, 2, PX>), dim3(grid), dim3(256), 0, st, ev0, ev1, 0, a);
+            else if (skip) hipExtLaunchKernelGGL((mma_kernel<HD, FMT, 4, true, EX, 1, PX>), dim3(grid), dim3(256), 0, st, ev0, ev1, 0, a);
+            else hipExtLaunchKernelGGL((mma_kernel<HD, FMT, 4, false, EX, 1, PX>), dim3(grid), dim3(256), 0, st, ev0, ev1, 0, a);
             break;
         case 8:
-            if (skip) hipExtLaunchKernelGGL((mma_kernel<HD, FMT, 8, true, EX>), dim3(grid), dim3(512), 0, st, ev0, ev1, 0, a);
-            else hipExtLaunchKernelGGL((mma_kernel<HD, FMT, 8, false, EX>), dim3(grid), dim3(512), 0, st, ev0, ev1, 0, a);
+            if (skip) hipExtLaunchKernelGGL((mma_kernel<HD, FMT, 8, true, EX, 1, PX>), dim3(grid), dim3(512), 0, st, ev0, ev1, 0, a);
+            else hipExtLaunchKernelGGL((mma_kernel<HD, FMT, 8, false, EX, 1, PX>), dim3(grid), dim3(512), 0, st, ev0, ev1, 0, a);
             break;
         default: return hipErrorInvalidValue;
     }
     return hipGetLastError();
 }
 
-static hipError_t launch_mma_128(int fmt, int nw, bool skip, int streams, const AttnArgs & a, uint32_t grid, hipStream_t st, hipEvent_t ev0,
-                                 hipEvent_t ev1) {
+static hipError_t launch_mma_128(int fmt, int nw, bool skip, int streams, bool px, const AttnArgs & a, uint32_t grid, hipStream_t st,
+                                 hipEvent_t ev0, hipEvent_t ev1) {
     const bool ex = a.qmode == 0;                                    // PA_QMODE_GGML over quantized K: exact block dots
+    if (px) {
+        if (!ex) return hipErrorInvalidValue;
+        if (fmt == 0) return launch_mma_fmt<128, 0, false, true>(nw, skip, streams, a, grid, st, ev0, ev1);
+        if (fmt == 1) return launch_mma_fmt<128, 1, true, true>(nw, skip, streams, a, grid, st, ev0, ev1);
+        if (fmt == 2) return launch_mma_fmt<128, 2, true, true>(nw, skip, streams, a, grid, st, ev0, ev1);
+        return hipErrorInvalidValue;
+    }
     if (fmt == 0) return launch_mma_fmt<128, 0, false>(nw, skip, streams, a, grid, st, ev0, ev1);
     if (fmt == 1) return ex ? launch_mma_fmt<128, 1, true>(nw, skip, streams, a, grid, st, ev0, ev1) : launch_mma_fmt<128, 1, false>(nw, skip, streams, a, grid, st, ev0, ev1);
     if (fmt == 2) return ex ? launch_mma_fmt<128, 2, true>(nw, skip, streams, a, grid, st, ev0, ev1) : launch_mma_fmt<128, 2, false>(nw, skip, streams, a, grid, st, ev0, ev1);
@@ -614,10 +644,10 @@ static hipError_t launch_mma_256(int fmt, bool skip, const AttnArgs & a, uint32_
     return hipErrorInvalidValue;
 }
 
-hipError_t launch_mma(int hd, int fmt, int nw, bool skip, int streams, const AttnArgs & a, uint32_t grid, hipStream_t st, hipEvent_t ev0,
-                      hipEvent_t ev1) {
-    if (hd == 128) return launch_mma_128(fmt, nw, skip, streams, a, grid, st, ev0, ev1);
-    if (hd == 256 && nw == 8) return launch_mma_256(fmt, skip, a, grid, st, ev0, ev1);
+hipError_t launch_mma(int hd, int fmt, int nw, bool skip, int streams, bool px, const AttnArgs & a, uint32_t grid, hipStream_t st,
+                      hipEvent_t ev0, hipEvent_t ev1) {
+    if (hd == 128) return launch_mma_128(fmt, nw, skip, streams, px, a, grid, st, ev0, ev1);
+    if (hd == 256 && nw == 8 && !px) return launch_mma_256(fmt, skip, a, grid, st, ev0, ev1);
     return hipErrorInvalidValue;
 }
 

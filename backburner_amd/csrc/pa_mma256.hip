@@ -59,7 +59,8 @@ __device__ __forceinline__ float m2_sum16(float v) {    // sum over lanes l and 
 // EX: exact block dots in ggml's query rounding (quantized K only). WPS: waves per SIMD the registers are sized for.
 // Instantiated at head dim 256; at 128 (three waves per SIMD, 167 VGPRs) the 16-row waves measured slower than the
 // 32-row mma_kernel on verify (157 against 111 us), each wave reading the whole K / V^T tile from LDS.
-template <int HD, int FMT, bool SKIP, bool EX, int WPS>
+// PX: probabilities to more than one fp16 rounding, as in mma_kernel.
+template <int HD, int FMT, bool SKIP, bool EX, int WPS, bool PX = false>
 __global__ __launch_bounds__(256, WPS) void mma256_kernel(const AttnArgs a) {
     static_assert(!EX || FMT != 0, "exact block dots need quantized K");
     using G2 = M2Geom<HD>;
@@ -323,16 +324,28 @@ __global__ __launch_bounds__(256, WPS) void mma256_kernel(const AttnArgs a) {
             }
         }
         mx = fmaxf(mx, tm);
-        mm_h8 P;
-        #pragma unroll
-        for (int kh = 0; kh < 2; kh++)
+        mm_h8 P, Pl;
+        if constexpr (PX) {
+            float ts[2] = {0.0f, 0.0f};
             #pragma unroll
-            for (int i = 0; i < 4; i++)
-                P[4 * kh + i] = (_Float16) __builtin_amdgcn_exp2f(EX ? S[kh][i] : fmaf(S[kh][i], sm, -mref));
-        #pragma unroll
-        for (int t = 0; t < 8; t += 2) {                             // the row sum of the fp16 P the PV MFMAs use
-            const mm_h2 pp = {P[t], P[t + 1]};
-            lsum = __builtin_amdgcn_fdot2(pp, one2, lsum, false);
+            for (int v = 0; v < 8; v++) {
+                const float e = __builtin_amdgcn_exp2f(EX ? S[v / 4][v % 4] : fmaf(S[v / 4][v % 4], sm, -mref));
+                ts[v & 1] += e;
+                P[v] = (_Float16) e;
+                if constexpr (FMT != 0) Pl[v] = (_Float16) (e - (float) P[v]);
+            }
+            lsum += ts[0] + ts[1];
+        } else {
+            #pragma unroll
+            for (int kh = 0; kh < 2; kh++)
+                #pragma unroll
+                for (int i = 0; i < 4; i++)
+                    P[4 * kh + i] = (_Float16) __builtin_amdgcn_exp2f(EX ? S[kh][i] : fmaf(S[kh][i], sm, -mref));
+            #pragma unroll
+            for (int t = 0; t < 8; t += 2) {                         // the row sum of the fp16 P the PV MFMAs use
+                const mm_h2 pp = {P[t], P[t + 1]};
+                lsum = __builtin_amdgcn_fdot2(pp, one2, lsum, false);
+            }
         }
         // ---- O^T += V^T P^T per 16-dim block: lane (g, L) of a transposing read addresses key 16 r + 4 g + L / 4,
         // dims 16 db + 4 (L % 4) .. +3; lane (g, s) then holds dim 16 db + s of keys 16 r + 4 g + j (j < 4)
@@ -343,6 +356,7 @@ __global__ __launch_bounds__(256, WPS) void mma256_kernel(const AttnArgs a) {
             const pa_h4 x1 = __builtin_bit_cast(pa_h4, __builtin_amdgcn_ds_read_tr16_b64_v4f16((MM_LDS mm_tr4 *) (vrow + 16 * M2_VST + 32 * db)));
             const mm_h8 va = __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7);
             O[db] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, P, O[db], 0, 0, 0);
+            if constexpr (PX && FMT != 0) O[db] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, Pl, O[db], 0, 0, 0);
         }
     };
     auto step = [&](uint32_t t, int r) {
@@ -409,8 +423,22 @@ static hipError_t launch_m16(int fmt, bool skip, bool ex, const AttnArgs & a, ui
     return hipGetLastError();
 }
 
+static hipError_t launch_m16_px(int fmt, bool skip, const AttnArgs & a, uint32_t grid, hipStream_t st, hipEvent_t ev0, hipEvent_t ev1) {
+    switch (fmt * 2 + (skip ? 1 : 0)) {
+        case 0: hipExtLaunchKernelGGL((mma256_kernel<256, 0, false, false, 2, true>), dim3(grid), dim3(256), 0, st, ev0, ev1, 0, a); break;
+        case 1: hipExtLaunchKernelGGL((mma256_kernel<256, 0, true, false, 2, true>), dim3(grid), dim3(256), 0, st, ev0, ev1, 0, a); break;
+        case 2: hipExtLaunchKernelGGL((mma256_kernel<256, 1, false, true, 2, true>), dim3(grid), dim3(256), 0, st, ev0, ev1, 0, a); break;
+        case 3: hipExtLaunchKernelGGL((mma256_kernel<256, 1, true, true, 2, true>), dim3(grid), dim3(256), 0, st, ev0, ev1, 0, a); break;
+        case 4: hipExtLaunchKernelGGL((mma256_kernel<256, 2, false, true, 2, true>), dim3(grid), dim3(256), 0, st, ev0, ev1, 0, a); break;
+        case 5: hipExtLaunchKernelGGL((mma256_kernel<256, 2, true, true, 2, true>), dim3(grid), dim3(256), 0, st, ev0, ev1, 0, a); break;
+        default: return hipErrorInvalidValue;
+    }
+    return hipGetLastError();
+}
+
 // ggml's query rounding over quantized K takes the exact block dots; f16 queries (and f16 K) the fp16 operands
-hipError_t launch_mma256(int fmt, bool skip, const AttnArgs & a, uint32_t grid, hipStream_t st, hipEvent_t ev0, hipEvent_t ev1) {
+hipError_t launch_mma256(int fmt, bool skip, bool px, const AttnArgs & a, uint32_t grid, hipStream_t st, hipEvent_t ev0, hipEvent_t ev1) {
+    if (px) return a.qmode == 0 ? launch_m16_px(fmt, skip, a, grid, st, ev0, ev1) : hipErrorInvalidValue;
     return launch_m16<256, 2>(fmt, skip, a.qmode == 0 && fmt != 0, a, grid, st, ev0, ev1);
 }
 

@@ -177,6 +177,38 @@ int pa_hip_normalise(const float * O, const float * m, const float * l, uint64_t
  * No code in the reference tree (the receiver is the fork's Metal flash attention). Returns 0 or -1. */
 int pa_hip_coattn_merge(const uint16_t * Oh, const float * lse, const float * O_loc, const float * m_loc, const float * l_loc,
                         uint64_t rows, uint32_t hd, float * out, float * lse_out, void * stream);
+/* Attention of a tree of drafted tokens over the cache (no counterpart in the reference, whose verify step takes a chain).
+ * The last n_nodes (1 .. 64) keys of the page table are the draft's own, node j the j-th of them; the keys before them are
+ * the context, which every row sees. Row g*n_nodes + t of a KV head (member g of the group, node t; rows a multiple of
+ * n_nodes, the order pa_hip_pack_q and pa_hip_append_rope write) sees node j's key where bit j of mask[t] is set: of a tree
+ * the node itself and its ancestors, of a chain the bits 0 .. t. mask: device uint64 [n_nodes], 8-byte aligned, read when
+ * the call runs, so that a captured call replays with the tree that is there then; bits from n_nodes on are ignored. What a
+ * row does not see never enters its result, whatever the bytes there (infinities, NaN). The reply format: Oh = f16(O / l)
+ * (fp16 bits [nkv][rows][hd], 8-byte aligned; 0 for a row that sees no key), lse = m + log l (fp32 [nkv][rows]; -inf there).
+ * PA_QMODE_GGML only. Returns 0 once enqueued, -1 on a bad argument (nothing enqueued). */
+int pa_hip_attn_tree(pa_hip_ws * ws, const pa_hip_shape * shape, const void * const * k_pages, const void * const * v_pages,
+                     const uint32_t * nkeys, int n_pages, uint32_t n_nodes, const uint64_t * mask, const float * Q,
+                     uint16_t * Oh, float * lse, void * stream);
+
+/* Types of the activations and logits that come from the model. */
+enum { PA_TYPE_F32 = 0, PA_TYPE_F16 = 1, PA_TYPE_BF16 = 2 };
+
+/* What sampled acceptance and scoring read off the logits, beside pa_hip_accept's argmax (no counterpart in the reference):
+ * row i of n_rows (0 .. 2^20) starts at element i*row_stride (>= vocab) of `logits` (type PA_TYPE_*, aligned to its size), and with
+ * y = scale * logits (scale > 0: 1 / temperature)
+ *   lse[i]          = log sum_j e^y_j
+ *   logp[i][g]      = y[given[i][g]] - lse[i], g < n_given (0 .. 1024); NaN for an id outside 0 .. vocab-1
+ *   entropy[i]      = -sum_j p_j log p_j, p_j = e^(y_j - lse[i])
+ *   top_id[i][k]    = the k-th largest logit's id, k < n_top (0 .. 32), ties by the lowest id (-0 == +0; NaN above all, as
+ *                     pa_hip_accept), and top_logp[i][k] its log probability; -1 and -inf past the vocabulary.
+ * A logit of -inf has probability 0 and adds nothing to the entropy. A row of -inf only has lse = -inf, log probabilities
+ * -inf and entropy 0; a NaN or +inf in a row makes its lse, log probabilities and entropy NaN. Outputs (device, 4-byte
+ * aligned): logp fp32 [n_rows][n_given], lse and entropy fp32 [n_rows], top_id int32 and top_logp fp32 [n_rows][n_top];
+ * given: device int32 [n_rows][n_given]. Pointers of empty arrays may be NULL, lse and entropy too when not wanted. Returns
+ * 0 once enqueued, -1 on a bad argument. */
+int pa_hip_logprobs(pa_hip_ws * ws, const void * logits, int type, int n_rows, int64_t vocab, int64_t row_stride, float scale,
+                    const int32_t * given, int n_given, int n_top, float * logp, float * lse, float * entropy,
+                    int32_t * top_id, float * top_logp, void * stream);
 /* ---------------------------------------------------------------- 4. KV ingest into HBM pages */
 /* APPEND (phone-attn.h:403-421) into device pages: n received rows of K and of V (rs bytes each, the shape's row
  * format) stored at positions pos0 .. pos0+n-1 of a layer whose page i holds positions [i*page_keys, (i+1)*page_keys)
@@ -195,6 +227,40 @@ int pa_hip_append_rows(const pa_hip_shape * shape, void * const * k_pages, void 
  * APPEND). Returns 0 or -1. */
 int pa_hip_append_f32(const pa_hip_shape * shape, void * const * k_pages, void * const * v_pages, int n_pages,
                       uint32_t page_keys, uint32_t pos0, const float * K, const float * V, uint32_t n, void * stream);
+/* The query / key norm and the position rotation of new tokens, with the append: for token t and each of its heads
+ *   y = x * weight / sqrt(mean(x^2) + eps)                         (weight NULL: y = x, no norm)
+ *   (a, b) -> (a cos - b sin, a sin + b cos) of th = positions[t] * inv_freq[i], i < n_rot / 2, on the pairs
+ *   (y[i], y[i + n_rot/2]), or with `interleaved` (y[2i], y[2i + 1]); dims from n_rot on are not rotated.
+ * Computed in fp64 and rounded to fp32 once (the angles of far positions need it, and the quantizer's borders then do not
+ * depend on the order of a sum). Keys go, quantized as pa_hip_append_f32 does, to positions pos0 .. pos0+n-1 of the pages,
+ * values too without norm and rotation; queries go as fp32 to q_out [nkv][rows][hd], row g*n + t = member g of the KV
+ * head's group (query head h*(rows/n) + g), token t: what pa_hip_attn and pa_hip_attn_tree read. */
+typedef struct pa_hip_rope {
+    const float * q_weight, * k_weight;   /* device fp32 [hd], or NULL: no norm */
+    const float * inv_freq;               /* device fp32 [n_rot / 2] */
+    float eps;
+    uint32_t n_rot;                       /* rotated dims of a head: even, 0 .. hd */
+    uint32_t interleaved;
+    uint32_t type;                        /* PA_TYPE_* of Q, K and V */
+    uint64_t q_stride, k_stride, v_stride; /* elements from one token to the next; 0 = packed (heads * hd) */
+} pa_hip_rope;
+/* Q [n][nkv*rows/n][hd], K and V [n][nkv][hd] (device, 4-byte aligned; strides even for the 16-bit types), positions device
+ * int32 [n], q_out 8-byte aligned; shape.rows a multiple of n. Q and q_out may both be NULL: keys and values only (rows is
+ * then ignored). Pages, rs and hb as for pa_hip_append_f32. No counterpart in the reference (the fork's model graph does
+ * this on the Mac). Returns 0 once enqueued, -1 on a bad argument (nothing enqueued). */
+int pa_hip_append_rope(const pa_hip_shape * shape, void * const * k_pages, void * const * v_pages, int n_pages,
+                       uint32_t page_keys, uint32_t pos0, const pa_hip_rope * rope, const void * Q, const void * K,
+                       const void * V, const int32_t * positions, uint32_t n, float * q_out, void * stream);
+/* Copies n rows (the nkv*hb bytes of the shape's row format) of K and of V in every one of n_layers layers: the row at position
+ * src_pos[i] (src_pos NULL: src_pos0 + i) to position dst_pos0 + i. src_k .. dst_v: host arrays of n_layers * src_pages (dst_pages)
+ * device pointers, layer-major, page p of a layer holding positions [p*page_keys, (p+1)*page_keys); src_pos: a
+ * host array, strictly increasing. Two uses: the accepted path of a draft tree moved together (src and dst the same tables;
+ * then src_pos[i] >= dst_pos0 + i, and each row arrives as it was before the call), and a fork filling its own copy of a
+ * page. A page may appear as source and as destination only at the same place of its table, and as destination once. No
+ * counterpart in the reference. Returns 0 once enqueued, -1 on a bad argument (nothing enqueued). */
+int pa_hip_copy_rows(const pa_hip_shape * shape, int n_layers, const void * const * src_k, const void * const * src_v,
+                     int src_pages, void * const * dst_k, void * const * dst_v, int dst_pages, uint32_t page_keys,
+                     const uint32_t * src_pos, uint32_t src_pos0, uint32_t dst_pos0, uint32_t n, void * stream);
 /* q8_0 / q4_0 quantizer of the library (ggml quantize_row_q8_0_ref / q4_0_ref semantics; the q8_0 one prepares Q in
  * PA_QMODE_GGML): n fp32 values (multiple of 32) at x (4-byte aligned) -> blocks at y (2-byte aligned), both device
  * pointers. Returns 0 or -1. */
