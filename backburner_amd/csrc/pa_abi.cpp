@@ -76,6 +76,7 @@ struct pa_hip_ws {
     // pa_hip_logprobs: a row's parts and their best keys
     float4 * lpart = nullptr; size_t lpart_cap = 0;
     unsigned long long * lkeys = nullptr; size_t lkeys_cap = 0;
+    unsigned int * lcount = nullptr; size_t lcount_cap = 0;
     // buffers replaced by a larger one: a graph captured earlier may still name them, so they live as long as the
     // workspace (growth at least doubles a buffer, so they hold less than the live ones)
     std::vector<void *> retired;
@@ -153,7 +154,7 @@ extern "C" void pa_hip_ws_destroy(pa_hip_ws * w) {
     (void) hipDeviceSynchronize();
     for (void * p : {(void *) w->po, (void *) w->pml, (void *) w->apart, (void *) w->acount, (void *) w->dk,
                      (void *) w->dv, (void *) w->dq, (void *) w->dout, (void *) w->ro, (void *) w->rml, (void *) w->lpart,
-                     (void *) w->lkeys})
+                     (void *) w->lkeys, (void *) w->lcount})
         (void) hipFree(p);
     for (void * p : w->retired) (void) hipFree(p);
     if (w->hst) (void) hipHostFree(w->hst);
@@ -847,14 +848,29 @@ extern "C" int pa_hip_logprobs(pa_hip_ws * ws, const void * logits, int type, in
         return bad("logits must be aligned to their type, the other arrays to 4 bytes");
     if (!ws) return bad("null workspace");
     LogprobArgs a;
-    a.seg = (int64_t) n_rows * ((vocab + 4095) / 4096) <= 1024 ? 4096 : 16384;
-    a.splits = (int) ((vocab + a.seg - 1) / a.seg);
+    const int64_t segs = (vocab + 4095) / 4096;
+    int64_t parts = std::min<int64_t>({segs, LP_MAX_PARTS, std::max<int64_t>(1, 1024 / n_rows)});
+    const int64_t per = (segs + parts - 1) / parts;
+    parts = (segs + per - 1) / per;
+    a.parts = (int) parts;
+    a.span = (uint32_t) (per * 4096);
     hipStream_t st = (hipStream_t) stream;
-    const size_t parts = (size_t) n_rows * a.splits;
-    if (!ensure(ws, ws->lpart, ws->lpart_cap, parts * sizeof(float4), st, true, "hipMalloc logprob parts")) return -1;
-    if (n_top > 0 && !ensure(ws, ws->lkeys, ws->lkeys_cap, parts * n_top * sizeof(unsigned long long), st, true, "hipMalloc logprob keys")) return -1;
+    if (parts > 1) {
+        const size_t n = (size_t) n_rows * parts;
+        const unsigned int * had = ws->lcount;
+        if (!ensure(ws, ws->lpart, ws->lpart_cap, n * sizeof(float4), st, true, "hipMalloc logprob parts") ||
+            !ensure(ws, ws->lkeys, ws->lkeys_cap, n * std::max(n_top, 1) * sizeof(unsigned long long), st, true, "hipMalloc logprob keys") ||
+            !ensure(ws, ws->lcount, ws->lcount_cap, (size_t) n_rows * sizeof(unsigned int), st, true, "hipMalloc logprob counters"))
+            return -1;
+        // once per allocation (never inside a capture, which refuses to grow); the kernel keeps them zero
+        if (ws->lcount != had && !hip_ok(hipMemsetAsync(ws->lcount, 0, ws->lcount_cap, st), "hipMemset logprob counters")) {
+            (void) hipFree(ws->lcount);
+            ws->lcount = nullptr; ws->lcount_cap = 0;
+            return -1;
+        }
+    }
     a.logits = logits; a.given = given; a.logp = logp; a.lse = lse; a.entropy = entropy; a.top_logp = top_logp; a.top_id = top_id;
-    a.part = ws->lpart; a.keys = ws->lkeys; a.vocab = vocab; a.stride = row_stride; a.scale = scale; a.type = type;
+    a.part = ws->lpart; a.keys = ws->lkeys; a.counter = ws->lcount; a.vocab = vocab; a.stride = row_stride; a.scale = scale; a.type = type;
     a.n_rows = n_rows; a.n_given = n_given; a.n_top = n_top;
     return hip_ok(launch_logprobs(a, st), "logprobs launch") ? 0 : -1;
 }

@@ -126,16 +126,19 @@ struct AcceptArgs {
 };
 hipError_t launch_accept(const AcceptArgs & a, hipStream_t st);
 
+constexpr int LP_MAX_PARTS = 64;    // workgroups of a row
 struct LogprobArgs {
     const void * logits;
     const int32_t * given;
     float * logp, * lse, * entropy, * top_logp;
     int32_t * top_id;
-    float4 * part;                  // [n_rows][splits] (max, sum, weighted sum, NaN seen) of a workgroup's part of a row
-    unsigned long long * keys;      // [n_rows][splits][n_top] its best keys (orderable value, ~index), 0 where it has none
+    float4 * part;                  // [n_rows][parts] (max, sum, weighted sum) of a workgroup's part of a row
+    unsigned long long * keys;      // [n_rows][parts][n_top] its best keys (orderable value, ~id), 0 where it has none
+    unsigned int * counter;         // [n_rows] workgroups done, zero between calls (the row's last one resets it)
     int64_t vocab, stride;
     float scale;
-    int type, n_rows, n_given, n_top, splits, seg;   // seg: values per workgroup
+    int type, n_rows, n_given, n_top, parts;
+    uint32_t span;                  // values per workgroup, a multiple of 4096
 };
 hipError_t launch_logprobs(const LogprobArgs & a, hipStream_t st);
 
