@@ -12,10 +12,15 @@
 // the last one to finish reading the parts in their order (so the result does not depend on which one it is).
 //
 // The best n_top: a value is a 64-bit key (order of the value, ~id), so the largest key is the largest value and among equal
-// ones the lowest id. A floor under the n_top best is kept: a thread whose maximum is not above it has no candidate, which is
-// all that most values cost. Candidates collect in LDS; where they might not fit, 64 groups of four threads take their best keys, and
-// the n_top-th largest of these is the new floor: at most n_top groups hold keys at or above it, so what is left always fits.
-// A candidate's place is the number of larger ones.
+// ones the lowest id. A wave collects candidates in LDS; sorted now and then (a key's place is the number of larger ones), their
+// n_top-th is a floor, and that a value lies below it (or below another wave's) is all that most values cost, without a barrier
+// in the loop. Before there is a floor, and where a lot of lanes pass it, the n_top-th largest of the lanes' maxima is one. At the
+// end the four waves' best are ranked.
+//
+// What bounds it: without alternatives the copy's rate (512 rows x 128,256 bf16 32 us, 4.1 TB/s; f32 51 us, 5.1 TB/s); with them the
+// vector instructions, about 5,600 per wave of 16 segments, half of them for the candidates (n_top 5 / 20: bf16 48 / 51 us, f32 59 /
+// 62). Candidates ranked by the whole workgroup at every segment with one took 99 us (n_top 20, bf16), kept sorted in the lanes by
+// insertion 60. A single row is latency: 5.6 us without, 10.8 with 5 alternatives of 151,936, in 38 workgroups.
 #include "pa_attn.h"
 #include "pa_common.h"
 
@@ -23,9 +28,8 @@ namespace pa_hip {
 
 typedef unsigned long long lp_key;
 
-constexpr int LP_TOP = 32, LP_NV = 16, LP_SEG = 256 * LP_NV;
-constexpr int LP_CAP = LP_TOP * 4 * LP_NV + LP_TOP;                  // candidates in LDS
-static_assert(LP_MAX_PARTS * LP_TOP <= LP_CAP, "the join takes every workgroup's best");
+constexpr int LP_NV = 16, LP_SEG = 256 * LP_NV;
+constexpr int LP_MORE = 24;                                          // new candidates of a wave after which they are sorted for a new floor
 
 __device__ __forceinline__ uint32_t lp_order(float x) {              // NaN above everything, -0 == +0
     uint32_t u = __builtin_bit_cast(uint32_t, x);
@@ -36,6 +40,13 @@ __device__ __forceinline__ lp_key lp_make_key(float x, uint32_t idx) { return ((
 __device__ __forceinline__ float lp_key_value(lp_key k) {
     const uint32_t u = (uint32_t) (k >> 32);
     return __builtin_bit_cast(float, u & 0x80000000u ? u & 0x7fffffffu : ~u);   // (of a NaN's key: a NaN)
+}
+
+// v_max_f32 as it is: fmaxf makes it two, the first against signalling NaN
+__device__ __forceinline__ float lp_max(float a, float b) {
+    float r;
+    asm("v_max_f32 %0, %1, %2" : "=v"(r) : "s"(b), "v"(a));
+    return r;
 }
 
 struct LpPart { float m, s, t; };
@@ -69,7 +80,7 @@ __device__ __forceinline__ LpPart lp_join_all(LpPart p, float c2, LpPart (&red)[
 // the row's part (any alignment: what lies past the range reads 0 and becomes -inf)
 template <typename T> struct LpLoad {
     static constexpr int VEC = 16 / (int) sizeof(T), NL = LP_NV / VEC;
-    static __device__ __forceinline__ uint32_t at(int i) { return (uint32_t) ((i / VEC) * 256 * VEC + threadIdx.x * VEC + i % VEC); }
+    static __device__ __forceinline__ uint32_t at(int i, uint32_t t) { return (uint32_t) (i / VEC) * 256 * VEC + t * VEC + i % VEC; }
     static __device__ __forceinline__ void load(pa_u4 (&r)[NL], const T * x, uint32_t n) {
         const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc((void *) x, (short) 0, (int) (n * sizeof(T)), 0x00020000);
         #pragma unroll
@@ -87,10 +98,12 @@ template <typename T> struct LpLoad {
         if (n < (uint32_t) LP_SEG) {
             // (a 16-bit value that ends the range in the middle of a dword is not in reach of its load)
             const float last = sizeof(T) == 2 && (n & 1) ? value(x[n - 1]) : 0.0f;
+            uint32_t t = threadIdx.x;
+            asm volatile("" : "+v"(t));                              // (the places computed here, not held in registers over the loop)
             #pragma unroll
             for (int i = 0; i < LP_NV; i++) {
-                if (sizeof(T) == 2 && (n & 1) && at(i) == n - 1) v[i] = last;
-                if (at(i) >= n) v[i] = -INFINITY;
+                if (sizeof(T) == 2 && (n & 1) && at(i, t) == n - 1) v[i] = last;
+                if (at(i, t) >= n) v[i] = -INFINITY;
             }
         }
     }
@@ -100,60 +113,136 @@ template <> __device__ __forceinline__ float LpLoad<_Float16>::value(_Float16 x)
 template <> __device__ __forceinline__ float LpLoad<uint16_t>::value(uint16_t x) { return __builtin_bit_cast(float, (uint32_t) x << 16); }
 
 struct LpShared {
-    __attribute__((aligned(16))) lp_key cand[LP_CAP];
-    __attribute__((aligned(16))) lp_key wbest[4][64], gbest[4][64];
-    lp_key out[LP_TOP];
+    __attribute__((aligned(16))) lp_key best[4][64];                 // per wave: scratch of a key per lane
+    __attribute__((aligned(16))) lp_key tops[4][32];                 // the waves' best, 0 where there are fewer
+    __attribute__((aligned(16))) float fval[4];                      // the values of the waves' floors
+    lp_key out[32];
     LpPart red[4];
-    int count;
     bool last;
 };
 
-// The n-th largest of the 64 groups' best keys (group l: lane l of each wave; mine: this thread's best, 0 for none), or 0
-// where fewer groups have one. Keys are distinct.
-__device__ __forceinline__ lp_key lp_floor(int n, lp_key mine, LpShared & sh) {
-    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-    sh.wbest[wave][lane] = mine;
-    __syncthreads();
-    lp_key g = 0;
-    #pragma unroll
-    for (int w = 0; w < 4; w++) g = sh.wbest[w][lane] > g ? sh.wbest[w][lane] : g;
-    sh.gbest[wave][lane] = g;                                        // every wave its own copy, read by it alone
-    __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
-    int above = 0;
-    #pragma unroll 16
-    for (int i = 0; i < 64; i++) above += sh.gbest[wave][i] > g;
-    const unsigned long long who = __ballot(g != 0 && above == n - 1);
-    return who ? sh.gbest[wave][__builtin_ctzll(who)] : 0;
+__device__ __forceinline__ void lp_wave_sync() { __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront"); }   // (DS runs in order)
+
+// the number of the wave's lanes below this one in `who`
+__device__ __forceinline__ int lp_below(unsigned long long who) {
+    return (int) __builtin_amdgcn_mbcnt_hi((uint32_t) (who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t) who, 0));
+}
+__device__ __forceinline__ lp_key lp_lane(lp_key k, int lane) {
+    return ((lp_key) (uint32_t) __builtin_amdgcn_readlane((int) (k >> 32), lane) << 32) | (uint32_t) __builtin_amdgcn_readlane((int) k, lane);
 }
 
-// The n best of the cur candidates, in order to sh.out (0 where there are fewer)
-__device__ __forceinline__ void lp_select(int n, int cur, LpShared & sh) {
-    constexpr int R = (LP_CAP + 255) / 256;
-    const int t = threadIdx.x;
-    if (cur > 128) {                                                 // few enough to be ranked by comparing all of them
-        lp_key k[R], mine = 0;
-        #pragma unroll
-        for (int i = 0; i < R; i++) {
-            k[i] = t + 256 * i < cur ? sh.cand[t + 256 * i] : 0;
-            mine = k[i] > mine ? k[i] : mine;
-        }
-        const lp_key fl = lp_floor(n, mine, sh);                     // (its barrier: every candidate is in registers)
-        if (t == 0) sh.count = 0;
-        __syncthreads();
-        if (mine >= fl)
-            #pragma unroll
-            for (int i = 0; i < R; i++)
-                if (k[i] && k[i] >= fl) sh.cand[atomicAdd(&sh.count, 1)] = k[i];
-        __syncthreads();
-        cur = sh.count;
+// the number of the wave's 64 keys above this lane's
+__device__ __forceinline__ int lp_above(lp_key mine, lp_key * best) {
+    best[threadIdx.x % 64] = mine;
+    lp_wave_sync();
+    int above = 0;
+    #pragma unroll 4
+    for (int i = 0; i < 64; i += 2) {
+        const pa_u4 x = *(const pa_u4 *) (best + i);
+        above += (((lp_key) x.y << 32) | x.x) > mine;
+        above += (((lp_key) x.w << 32) | x.z) > mine;
     }
-    if (t < n) sh.out[t] = 0;
+    lp_wave_sync();
+    return above;
+}
+// of 32-bit orders, which may be equal (0: none), the largest that at least n lanes reach, or 0
+__device__ __forceinline__ uint32_t lp_nth_value(int n, uint32_t mine, lp_key * best) {
+    uint32_t * b = (uint32_t *) best;
+    b[threadIdx.x % 64] = mine;
+    lp_wave_sync();
+    int above = 0;
+    #pragma unroll 4
+    for (int i = 0; i < 64; i += 4) {
+        const pa_u4 x = *(const pa_u4 *) (b + i);
+        above += (x.x > mine) + (x.y > mine) + (x.z > mine) + (x.w > mine);
+    }
+    // of the lanes that fewer than n pass, the one that most pass
+    int w = mine != 0 && above < n ? above : -1;
+    const int in = __builtin_popcountll(__ballot(w >= 0));
+    #pragma unroll
+    for (int off = 32; off > 0; off >>= 1) w = max(w, __shfl_xor(w, off));
+    const unsigned long long who = __ballot(mine != 0 && above == w);
+    lp_wave_sync();
+    return in < n ? 0 : (uint32_t) __builtin_amdgcn_readlane((int) mine, __builtin_ctzll(who));
+}
+
+__device__ __host__ constexpr int lp_room(int n) { return 16 * n + 64; }   // of a wave's list: n lanes' values, or a quarter of the parts' best
+
+// A wave's candidates: list[0 .. count - 1] in LDS, room for lp_room(n)
+struct LpTop {
+    lp_key * list, * best;                                           // the wave's LDS: lp_room(n) and 64 keys
+    int n, count = 0;
+    lp_key floor = 0;                                                // n of the candidates reach it (0: there are fewer)
+    float fval = -INFINITY;                                          // its value; -inf without one
+
+    __device__ __forceinline__ void push(bool want, lp_key k) {     // by the whole wave
+        const unsigned long long who = __ballot(want);
+        if (want) list[count + lp_below(who)] = k;
+        count += __builtin_popcountll(who);
+    }
+    __device__ __forceinline__ void set_floor(lp_key k) {
+        floor = k;
+        fval = k ? lp_key_value(k) : -INFINITY;
+    }
+    // the n best, sorted, in list[0 .. n - 1], and no others
+    __device__ __forceinline__ void sort() {
+        const int lane = threadIdx.x % 64;
+        lp_wave_sync();
+        if (count > 64) {                                            // those that reach the n-th largest of the lanes' best, in place
+            const int had = count;
+            lp_key mine = 0;
+            for (int i = lane; i < had; i += 64) mine = list[i] > mine ? list[i] : mine;
+            const unsigned long long who = __ballot(lp_above(mine, best) == n - 1 && mine != 0);
+            const lp_key fl = who ? lp_lane(mine, __builtin_ctzll(who)) : 1;
+            count = 0;
+            for (int i = 0; i < had; i += 64) {                      // (no write passes what has been read)
+                const lp_key k = i + lane < had ? list[i + lane] : 0;
+                lp_wave_sync();
+                push(k >= fl, k);
+            }
+            lp_wave_sync();
+        }
+        if (count <= 64) {                                           // one key per lane, its place the number of larger ones
+            const lp_key k = lane < count ? list[lane] : 0;
+            const int place = lp_above(k, best);
+            if (k && place < n) list[place] = k;
+            count = min(count, n);
+        } else {                                                     // rare (the best in few lanes): one after the other, sorted in
+            lp_key top = 0;                                          // the lanes' registers
+            for (int i = 0; i < count; i += 64) {
+                lp_key k = i + lane < count ? list[i + lane] : 0, fl = lp_lane(top, n - 1);
+                for (unsigned long long b = __ballot(k > fl); b; b = __ballot(k > fl)) {
+                    const lp_key c = lp_lane(k, __builtin_ctzll(b));
+                    const int place = __builtin_popcountll(__ballot(top > c));
+                    const lp_key up = __shfl_up(top, 1);
+                    top = lane < place ? top : lane == place ? c : up;
+                    k = k == c ? 0 : k;
+                    fl = lp_lane(top, n - 1);
+                }
+            }
+            if (lane < n) list[lane] = top;
+            count = n;
+        }
+        lp_wave_sync();
+        set_floor(count == n ? list[n - 1] : 0);
+    }
+};
+
+// The n best of the four waves' best, in order to sh.out (0 where there are fewer)
+__device__ __forceinline__ void lp_rank(LpTop & l, LpShared & sh) {
+    const int t = threadIdx.x;
+    l.sort();
+    if (t % 64 < 32) sh.tops[t / 64][t % 64] = t % 64 < l.count ? l.list[t % 64] : 0;
+    if (t < l.n) sh.out[t] = 0;
     __syncthreads();
-    for (int i = t; i < cur; i += 256) {
-        const lp_key k = sh.cand[i];
+    const int w = t / 32, i = t % 32;
+    if (w < 4 && i < l.n) {
+        const lp_key k = sh.tops[w][i];
         int place = 0;
-        for (int j = 0; j < cur; j++) place += sh.cand[j] > k;
-        if (k && place < n) sh.out[place] = k;
+        #pragma unroll 2
+        for (int j = 0; j < l.n; j++)
+            place += (sh.tops[0][j] > k) + (sh.tops[1][j] > k) + (sh.tops[2][j] > k) + (sh.tops[3][j] > k);
+        if (k && place < l.n) sh.out[place] = k;
     }
     __syncthreads();
 }
@@ -166,12 +255,14 @@ template <typename T> __global__ __launch_bounds__(256) void logprob_kernel(cons
     const uint32_t j0 = (uint32_t) w * a.span, j1 = (uint32_t) min((int64_t) a.vocab, (int64_t) j0 + a.span);
     const float c2 = a.scale * PA_LOG2E;
     LpPart p = {-INFINITY, 0.0f, 0.0f};
-    lp_key floor = 0;
-    float fval = 0.0f;
-    int cur = 0;                                                     // candidates in LDS
+    extern __shared__ __attribute__((aligned(16))) lp_key lists[];   // [4][lp_room(n_top)], then [4][LP_NV / 4][64] x 4 floats
+    pa_f4 * vals = (pa_f4 *) (lists + 4 * lp_room(a.n_top)) + 64 * (LP_NV / 4) * (t / 64) + t % 64;
+    LpTop top;
+    top.n = a.n_top; top.list = lists + lp_room(a.n_top) * (t / 64); top.best = sh.best[t / 64];
+    if (t < 4) sh.fval[t] = -INFINITY;
+    if (a.n_top > 0) __syncthreads();
     pa_u4 r[L::NL];
     L::load(r, x + j0, min(j1 - j0, (uint32_t) LP_SEG));
-    if (t == 0) sh.count = 0;
     for (uint32_t j = j0; j < j1; j += LP_SEG) {
         const uint32_t n = min(j1 - j, (uint32_t) LP_SEG);
         float v[LP_NV];
@@ -189,41 +280,47 @@ template <typename T> __global__ __launch_bounds__(256) void logprob_kernel(cons
         for (int i = 0; i < LP_NV; i++) {
             const float d = v[i] - ms, e = __builtin_amdgcn_exp2f(d * c2);
             p.s += e;
-            p.t = fmaf(e, fmaxf(d, -3e38f), p.t);                    // -inf: e = 0, and 0 * (a number) = 0
+            p.t = fmaf(e, lp_max(d, -3e38f), p.t);                   // -inf: e = 0, and 0 * (a number) = 0
         }
         if (a.n_top == 0) continue;
-        const bool any = L::at(0) < n, nan = p.s != p.s;             // (at(0): this thread's first value)
-        auto hits = [&] { return any && (floor == 0 || nan || mt > fval); };
-        int h = __syncthreads_count(hits());
+        const bool any = L::at(0, t) < n, nan = p.s != p.s;             // (at(0): this thread's first value)
+        // what lies below another wave's floor is not wanted either (equal values may be: their ids can be lower here)
+        const pa_f4 fo = *(const volatile pa_f4 *) sh.fval;
+        float low = fmaxf(fmaxf(fo.x, fo.y), fmaxf(fo.z, fo.w));
+        bool hit = any && (nan || ((top.floor == 0 || mt > top.fval) && !(mt < low)));
+        const int h = __builtin_popcountll(__ballot(hit));
         if (h == 0) continue;
-        auto each = [&](auto f) {
-            #pragma unroll
-            for (int i = 0; i < LP_NV; i++)
-                if (L::at(i) < n) f(lp_make_key(v[i], j + L::at(i)));
-        };
-        if (cur + h * LP_NV > LP_CAP) {
-            if (cur > 0) {                                           // the n_top best so far, and their last one as the floor
-                lp_select(a.n_top, cur, sh);
-                if (t < a.n_top) sh.cand[t] = sh.out[t];
-                cur = a.n_top;
-                const lp_key k = sh.out[a.n_top - 1];
-                if (k > floor) { floor = k; fval = lp_key_value(k); }
-                if (t == 0) sh.count = cur;
-                h = __syncthreads_count(hits());
-            }
-            if (cur + h * LP_NV > LP_CAP) {
-                lp_key mine = 0;
-                if (hits()) each([&](lp_key k) { mine = k > mine ? k : mine; });
-                const lp_key k = lp_floor(a.n_top, mine, sh);
-                if (k > floor) { floor = k; fval = lp_key_value(k); }
-            }
+        if (h > top.n) {                                             // not only the lanes that matter: a floor from their maxima
+            const uint32_t mine = hit ? (nan ? 0xffffffffu : lp_order(mt)) : 0u;
+            const uint32_t o = lp_nth_value(top.n, mine, top.best);
+            hit = hit && mine >= o;
+            const float ov = lp_key_value((lp_key) o << 32);
+            low = ov > low ? ov : low;
         }
-        if (any && (floor == 0 || nan || mt >= fval))
-            each([&](lp_key k) { if (k >= floor) sh.cand[atomicAdd(&sh.count, 1)] = k; });
-        __syncthreads();
-        cur = sh.count;
+        low = fmaxf(low, top.fval);
+        // a lane's candidates (a NaN is one), one of each lane at a time: bits of their places, the values by LDS
+        uint32_t left = 0;
+        #pragma unroll
+        for (int i = LP_NV - 1; i >= 0; i--) left = left + left + (v[i] < low ? 0u : 1u);
+        left = hit ? left : 0;
+        #pragma unroll
+        for (int u = 0; u < LP_NV / 4; u++) vals[64 * u] = (pa_f4){v[4 * u], v[4 * u + 1], v[4 * u + 2], v[4 * u + 3]};
+        lp_wave_sync();
+        while (__ballot(left != 0)) {
+            const uint32_t i = __builtin_ctz(left | 1u << 31) & (LP_NV - 1);
+            const float val = ((const float *) (vals + 64 * (i / 4)))[i % 4];
+            const uint32_t at = L::at(i, t);
+            const lp_key k = left != 0 && at < n ? lp_make_key(val, j + at) : 0;
+            left &= left - 1;
+            if (top.count + 64 > lp_room(top.n)) top.sort();
+            top.push(k > top.floor, k);
+        }
+        if (j + LP_SEG < j1 && top.count >= (top.floor == 0 ? top.n : top.n + LP_MORE)) {
+            top.sort();
+            if (t % 64 == 0) sh.fval[t / 64] = top.fval;
+        }
     }
-    if (a.n_top > 0) lp_select(a.n_top, cur, sh);
+    if (a.n_top > 0) lp_rank(top, sh);
     p = lp_join_all(p, c2, sh.red);
 
     if (a.parts > 1) {
@@ -252,9 +349,14 @@ template <typename T> __global__ __launch_bounds__(256) void logprob_kernel(cons
             p = LpPart{ms.x, ms.y, tt.x};
         }
         const int nk = a.parts * a.n_top;
-        for (int i = t; i < nk; i += 256) sh.cand[i] = __hip_atomic_load(&keys[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        top.count = 0; top.floor = 0;                                // a quarter of the keys per wave
+        for (int i0 = 64 * (t / 64); i0 < nk; i0 += 256) {
+            const int i = i0 + t % 64;
+            const lp_key k = i < nk ? __hip_atomic_load(&keys[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0;
+            top.push(k != 0, k);
+        }
         p = lp_join_all(p, c2, sh.red);
-        if (a.n_top > 0) lp_select(a.n_top, nk, sh);
+        if (a.n_top > 0) lp_rank(top, sh);
     }
 
     const bool bad = p.s != p.s || p.m == INFINITY, none = p.m == -INFINITY;
@@ -277,11 +379,12 @@ template <typename T> __global__ __launch_bounds__(256) void logprob_kernel(cons
 
 hipError_t launch_logprobs(const LogprobArgs & a, hipStream_t st) {
     const dim3 grid((uint32_t) a.n_rows * a.parts);
+    const size_t lds = a.n_top ? (size_t) 4 * lp_room(a.n_top) * sizeof(lp_key) + LP_SEG * sizeof(float) : 0;   // at most 34 KB
     if (a.n_rows == 0) return hipSuccess;
     if (a.parts > LP_MAX_PARTS || (int64_t) a.parts * a.span < a.vocab || (int64_t) (a.parts - 1) * a.span >= a.vocab) return hipErrorInvalidValue;
-    if (a.type == PA_TYPE_F32) hipLaunchKernelGGL(logprob_kernel<float>, grid, dim3(256), 0, st, a);
-    else if (a.type == PA_TYPE_F16) hipLaunchKernelGGL(logprob_kernel<_Float16>, grid, dim3(256), 0, st, a);
-    else if (a.type == PA_TYPE_BF16) hipLaunchKernelGGL(logprob_kernel<uint16_t>, grid, dim3(256), 0, st, a);
+    if (a.type == PA_TYPE_F32) hipLaunchKernelGGL(logprob_kernel<float>, grid, dim3(256), lds, st, a);
+    else if (a.type == PA_TYPE_F16) hipLaunchKernelGGL(logprob_kernel<_Float16>, grid, dim3(256), lds, st, a);
+    else if (a.type == PA_TYPE_BF16) hipLaunchKernelGGL(logprob_kernel<uint16_t>, grid, dim3(256), lds, st, a);
     else return hipErrorInvalidValue;
     return hipGetLastError();
 }
