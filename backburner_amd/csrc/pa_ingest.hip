@@ -9,6 +9,8 @@
 // The plain APPEND copy (phone-attn.h:403-421) is a device copy per page segment, issued by the host code.
 //
 // 16 lanes per 32-value block (details below). The work is a byte stream: HBM-bound, a few µs for a 512-token APPEND.
+#include <algorithm>
+
 #include "pa_attn.h"
 #include "pa_common.h"
 
@@ -122,31 +124,97 @@ __global__ __launch_bounds__(256) void append_quant_kernel(const AppendArgs a) {
 }
 
 // ---------------------------------------------------------------- norm, rotation and append in one pass
-// Two consecutive values of a head as fp64 (exact for all three types)
-__device__ __forceinline__ void rope_load2(int type, const void * p, double & x0, double & x1) {
-    if (type == PA_TYPE_F32) {
-        const float2 v = *(const float2 *) p;
-        x0 = v.x; x1 = v.y;
-    } else {
-        const uint32_t u = *(const uint32_t *) p;
-        if (type == PA_TYPE_F16) {
-            x0 = pa_f16_bits_to_f32((uint16_t) u); x1 = pa_f16_bits_to_f32((uint16_t) (u >> 16));
-        } else {
-            x0 = __builtin_bit_cast(float, u << 16); x1 = __builtin_bit_cast(float, u & 0xffff0000u);
-        }
+// A 32-block over 8 lanes, lane l (of the 8) holding values 4l .. 4l+3: the bytes of quant_block16, from the same expressions
+template <int CTRL> __device__ __forceinline__ float ing_dpp_f(float v) { return __builtin_bit_cast(float, ing_dpp<CTRL>(__builtin_bit_cast(uint32_t, v))); }
+__device__ __forceinline__ void quant_block8(int fmt, const float (&x)[4], int l, uint8_t * o) {
+    #pragma clang fp contract(off)
+    if (fmt == 0) {
+        const pa_h4 h = {(_Float16) x[0], (_Float16) x[1], (_Float16) x[2], (_Float16) x[3]};
+        __builtin_memcpy(o + 8 * l, &h, 8);
+        return;
     }
+    float amax = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
+    amax = fmaxf(amax, ing_dpp_f<0xb1>(amax));
+    amax = fmaxf(amax, ing_dpp_f<0x4e>(amax));
+    amax = fmaxf(amax, ing_dpp_f<0x141>(amax));                      // row_half_mirror: lane ^ 7
+    if (fmt == 1) {
+        const float d = amax / 127.0f;
+        const float id = d != 0.0f ? 1.0f / d : 0.0f;
+        uint32_t w = 0;
+        #pragma unroll
+        for (int e = 0; e < 4; e++) w |= ((uint32_t) (int) roundf(x[e] * id) & 0xffu) << (8 * e);
+        __builtin_memcpy(o + 2 + 4 * l, &w, 4);
+        if (l == 0) *(uint16_t *) o = __builtin_bit_cast(uint16_t, (_Float16) d);
+        return;
+    }
+    // the first value of the largest magnitude: the least (place, sign) among those that have it
+    uint32_t at = 64;
+    #pragma unroll
+    for (int e = 3; e >= 0; e--) at = fabsf(x[e]) == amax ? (uint32_t) (4 * l + e) * 2 + (__builtin_bit_cast(uint32_t, x[e]) >> 31) : at;
+    at = min(at, ing_dpp<0xb1>(at));
+    at = min(at, ing_dpp<0x4e>(at));
+    at = min(at, ing_dpp<0x141>(at));
+    const float mx = amax == 0.0f ? 0.0f : (at & 1) ? -amax : amax;
+    const float d = mx / -8.0f;
+    const float id = d != 0.0f ? 1.0f / d : 0.0f;
+    const uint16_t dh = d == 0.0f ? (uint16_t) ((__builtin_bit_cast(uint32_t, mx) >> 16) & 0x8000u) ^ 0x8000u   // (see quant_block16)
+                                  : __builtin_bit_cast(uint16_t, (_Float16) d);
+    uint32_t w = 0;
+    #pragma unroll
+    for (int e = 0; e < 4; e++) {
+        const int q = (int8_t) (x[e] * id + 8.5f);
+        w |= ((uint32_t) (q > 15 ? 15 : q) & 0xffu) << (8 * e);
+    }
+    w |= ing_dpp<0x104>(w) << 4;                                     // row_shl:4: values 16 on, four lanes further
+    if (l < 4) __builtin_memcpy(o + 2 + 4 * l, &w, 4);
+    if (l == 0) *(uint16_t *) o = dh;
 }
 
-// Workgroup = one token and a share of its heads (queries, then keys, then values), a head per wave at a time: lane l holds dims
-// 2l, 2l + 1 (and 128 more of head dim 256), a quantizer's block then sits in 16 lanes.
-template <int HD>
+__device__ __forceinline__ double rope_join(uint32_t lo, uint32_t hi) { return __builtin_bit_cast(double, (uint64_t) hi << 32 | lo); }
+template <int CTRL> __device__ __forceinline__ double rope_dpp(double v) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    return rope_join(ing_dpp<CTRL>((uint32_t) u), ing_dpp<CTRL>((uint32_t) (u >> 32)));
+}
+
+// Workgroup = one token and a share of its heads (queries, then keys, then values); a wave takes HPW heads at a time, HD / 8 lanes
+// each: lane q holds dims 4q .. 4q+3 and HD/2 + 4q .. +3, so that a rotation's pairs lie in one lane where the whole head is
+// rotated (MODE 0: halves, 1: interleaved), 16 bytes are loaded at once and a quantizer's block is 8 lanes. MODE 2: a part of the
+// head rotated, the pairs through LDS. The angles' cos and sin are computed once per workgroup.
+//
+// What bounds it: for long chunks HBM and the fp64 conversions and products about alike (2,048 tokens x 80 heads x 128 of bf16: 114 MB,
+// 22 us at the copy rate, and 940 vector instructions in each of 8,192 waves; 31.5 us. A wave per head with two dims a lane took
+// 76 us: twelve lane swaps for the sum of each head, the sines of each four heads anew); launch and the fp64 sine for short ones.
+template <int HD, int MODE>
 __global__ __launch_bounds__(256) void append_rope_kernel(const RopeArgs r) {
-    constexpr int NP = HD / 128;                                     // value pairs per lane
-    __shared__ double cs[HD / 2][2];                                 // cos, sin of the token's angles
-    __shared__ double ys[4][HD];                                     // a wave's normed head, for the pairs that span lanes
-    const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64;
+    constexpr int LPH = HD / 8, HPW = 64 / LPH, H2 = HD / 2;
+    __shared__ __attribute__((aligned(16))) double cs[H2][2];        // cos, sin of the token's angles
+    __shared__ double ys[MODE == 2 ? 4 : 1][MODE == 2 ? HPW : 1][MODE == 2 ? HD : 1];
+    const int tid = threadIdx.x, lane = tid % 64, wave = __builtin_amdgcn_readfirstlane(tid / 64), q = lane % LPH, hw = lane / LPH;
     const uint32_t j = blockIdx.y, t = r.t0 + j, half = r.n_rot / 2;
-    const uint32_t nq = r.q ? r.a.nkv * r.gqa : 0, nkv = r.a.nkv, heads = nq + 2 * nkv;
+    const uint32_t nq = r.q ? r.a.nkv * r.gqa : 0, nkv = r.a.nkv;
+    const bool f32 = r.type == PA_TYPE_F32;
+    // an item: HPW heads of one kind (query 0, key 1, value 2), the last one of a kind maybe fewer
+    const uint32_t iq = (nq + HPW - 1) / HPW, ik = (nkv + HPW - 1) / HPW, items = iq + 2 * ik;
+    auto kind_of = [&](uint32_t it) { return it < iq ? 0 : it < iq + ik ? 1 : 2; };
+    auto head_of = [&](uint32_t it) { return (it < iq ? it : it < iq + ik ? it - iq : it - iq - ik) * HPW + hw; };
+    // a head's 8 values of this lane as they come: two times 16 bytes of f32, 8 of the others
+    auto load = [&](uint32_t it, pa_u4 (&x)[2]) {
+        const int kind = kind_of(it);
+        const uint32_t h = head_of(it);
+        const size_t at = (size_t) t * (kind == 0 ? r.qst : kind == 1 ? r.kst : r.vst) + (size_t) h * HD + 4 * q;
+        const void * src = kind == 0 ? r.q : kind == 1 ? r.k : r.v;
+        x[0] = x[1] = (pa_u4){0u, 0u, 0u, 0u};
+        if (h >= (kind == 0 ? nq : nkv)) return;
+        #pragma unroll
+        for (int s = 0; s < 2; s++) {
+            if (f32) __builtin_memcpy(&x[s], (const float *) src + at + s * H2, 16);
+            else __builtin_memcpy(&x[s], (const uint16_t *) src + at + s * H2, 8);
+        }
+    };
+    const uint32_t step = gridDim.x * 4;
+    uint32_t it = blockIdx.x * 4 + wave;
+    pa_u4 raw[2];
+    if (it < items) load(it, raw);
     if ((uint32_t) tid < half) {
         // the angle in turns: th = pos * f is exact (24 + 29 bits), 1 / (2 pi) in two parts, the whole turns taken out in between
         const double th = (double) r.pos[t] * (double) r.freq[tid];
@@ -160,53 +228,79 @@ __global__ __launch_bounds__(256) void append_rope_kernel(const RopeArgs r) {
     __syncthreads();
     const uint32_t p = r.a.off0 + j, pg = p < r.a.page_keys ? 0u : p / r.a.page_keys;
     const size_t prow = (size_t) (p - pg * r.a.page_keys) * r.a.rs;
-    for (uint32_t hj = blockIdx.x * 4 + wave; hj < heads; hj += gridDim.x * 4) {
-        const int kind = hj < nq ? 0 : hj < nq + nkv ? 1 : 2;        // query, key, value (uniform in the wave)
-        const uint32_t h = kind == 0 ? hj : kind == 1 ? hj - nq : hj - nq - nkv;
-        const size_t at = (size_t) t * (kind == 0 ? r.qst : kind == 1 ? r.kst : r.vst) + (size_t) h * HD + 2 * lane;
-        const uint8_t * src = (const uint8_t *) (kind == 0 ? r.q : kind == 1 ? r.k : r.v) + at * (r.type == PA_TYPE_F32 ? 4 : 2);
-        double y[2 * NP];
+    double wd[8];                                                    // the norm's weights of kind wk
+    int wk = -1;
+    for (; it < items; it += step) {
+        const int kind = kind_of(it);
+        const uint32_t h = head_of(it);
+        double y[8];
         #pragma unroll
-        for (int i = 0; i < NP; i++) rope_load2(r.type, src + (size_t) i * 128 * (r.type == PA_TYPE_F32 ? 4 : 2), y[2 * i], y[2 * i + 1]);
-        if (kind < 2) {
-            const float * w = kind == 0 ? r.qw : r.kw;
-            if (w) {
-                double ss = 0;
+        for (int i = 0; i < 8; i++) {
+            const uint32_t w = raw[i / 4][f32 ? i % 4 : (i % 4) / 2];
+            const uint16_t u = (uint16_t) (i & 1 ? w >> 16 : w);
+            y[i] = f32 ? __builtin_bit_cast(float, w) : r.type == PA_TYPE_F16 ? pa_f16_bits_to_f32(u) : __builtin_bit_cast(float, (uint32_t) u << 16);
+        }
+        if (it + step < items) load(it + step, raw);
+        const float * w = kind == 0 ? r.qw : kind == 1 ? r.kw : nullptr;
+        if (w) {
+            if (kind != wk) {
+                float wv[8];
+                __builtin_memcpy(wv, w + 4 * q, 16);
+                __builtin_memcpy(wv + 4, w + H2 + 4 * q, 16);
                 #pragma unroll
-                for (int i = 0; i < 2 * NP; i++) ss += y[i] * y[i];
-                #pragma unroll
-                for (int off = 32; off > 0; off >>= 1) ss += __shfl_xor(ss, off);
-                const double f = 1.0 / sqrt(ss / HD + (double) r.eps);
-                #pragma unroll
-                for (int i = 0; i < 2 * NP; i++) y[i] *= f * (double) w[128 * (i / 2) + 2 * lane + (i & 1)];
+                for (int i = 0; i < 8; i++) wd[i] = wv[i];
+                wk = kind;
             }
-            if (half > 0) {
-                #pragma unroll
-                for (int i = 0; i < 2 * NP; i++) ys[wave][128 * (i / 2) + 2 * lane + (i & 1)] = y[i];
-                __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");   // one wave's LDS operations run in order
-                #pragma unroll
-                for (int i = 0; i < 2 * NP; i++) {
-                    const uint32_t d = 128 * (i / 2) + 2 * lane + (i & 1);
-                    if (d < r.n_rot) {
-                        const bool first = r.interleaved ? (d & 1) == 0 : d < half;
-                        const uint32_t f = r.interleaved ? d / 2 : first ? d : d - half;
-                        const double o = ys[wave][r.interleaved ? d ^ 1 : first ? d + half : d - half];
-                        y[i] = first ? y[i] * cs[f][0] - o * cs[f][1] : o * cs[f][1] + y[i] * cs[f][0];
-                    }
+            double ss = 0;
+            #pragma unroll
+            for (int i = 0; i < 8; i++) ss = fma(y[i], y[i], ss);
+            ss += rope_dpp<0xb1>(ss);
+            ss += rope_dpp<0x4e>(ss);
+            ss += rope_dpp<0x141>(ss);
+            ss += rope_dpp<0x140>(ss);                               // row_mirror: lane ^ 15
+            if constexpr (LPH == 32) ss += __shfl_xor(ss, 16);
+            const double f = rsqrt(ss / HD + (double) r.eps);
+            #pragma unroll
+            for (int i = 0; i < 8; i++) y[i] *= f * wd[i];
+        }
+        if (MODE == 2 && half > 0) {
+            #pragma unroll
+            for (int i = 0; i < 8; i++) ys[wave][hw][(i / 4) * H2 + 4 * q + i % 4] = y[i];
+            __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");   // one wave's LDS operations run in order
+            #pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const uint32_t d = (i / 4) * H2 + 4 * q + i % 4;
+                if (kind < 2 && d < r.n_rot) {
+                    const bool first = r.interleaved ? (d & 1) == 0 : d < half;
+                    const uint32_t f = r.interleaved ? d / 2 : first ? d : d - half;
+                    const double o = ys[wave][hw][r.interleaved ? d ^ 1 : first ? d + half : d - half];
+                    y[i] = first ? y[i] * cs[f][0] - o * cs[f][1] : o * cs[f][1] + y[i] * cs[f][0];
                 }
-                __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+            }
+            __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+        }
+        if constexpr (MODE < 2) {
+            if (kind < 2) {
+                #pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int ia = MODE == 0 ? e : 2 * e, ib = MODE == 0 ? 4 + e : 2 * e + 1;
+                    const int f = MODE == 0 ? 4 * q + e : (e / 2) * (HD / 4) + 2 * q + e % 2;
+                    const double a = y[ia], b = y[ib], c = cs[f][0], s = cs[f][1];
+                    y[ia] = a * c - b * s;
+                    y[ib] = a * s + b * c;
+                }
             }
         }
+        if (h >= (kind == 0 ? nq : nkv)) continue;                   // whole groups of lanes
         #pragma unroll
-        for (int i = 0; i < NP; i++) {
-            const float x0 = (float) y[2 * i], x1 = (float) y[2 * i + 1];
+        for (int k = 0; k < 2; k++) {
+            const float x[4] = {(float) y[4 * k], (float) y[4 * k + 1], (float) y[4 * k + 2], (float) y[4 * k + 3]};
             if (kind == 0) {
-                const size_t row = ((size_t) (h / r.gqa) * r.gqa + h % r.gqa) * r.n + t;
-                *(float2 *) (r.qout + row * HD + 128 * i + 2 * lane) = make_float2(x0, x1);
+                __builtin_memcpy(r.qout + ((size_t) h * r.n + t) * HD + k * H2 + 4 * q, x, 16);   // (head h = KV head * gqa + member)
             } else {
                 uint8_t * o = (kind == 1 ? r.a.kdst[pg] : r.a.vdst[pg]) + prow + (size_t) h * r.a.hb;
                 const uint32_t bb = r.a.fmt == 1 ? 34 : r.a.fmt == 2 ? 18 : 64;
-                quant_block16(r.a.fmt, x0, x1, lane % 16, o + (4 * i + lane / 16) * bb);
+                quant_block8(r.a.fmt, x, q % 8, o + (k * (HD / 64) + q / 8) * bb);
             }
         }
     }
@@ -242,11 +336,19 @@ hipError_t launch_append(bool from_f32, const AppendArgs & a, hipStream_t st) {
     return hipGetLastError();
 }
 
+template <int HD> static void launch_rope_hd(const RopeArgs & r, const dim3 & grid, hipStream_t st) {
+    if (r.n_rot == HD && !r.interleaved) hipLaunchKernelGGL((append_rope_kernel<HD, 0>), grid, dim3(256), 0, st, r);
+    else if (r.n_rot == HD) hipLaunchKernelGGL((append_rope_kernel<HD, 1>), grid, dim3(256), 0, st, r);
+    else hipLaunchKernelGGL((append_rope_kernel<HD, 2>), grid, dim3(256), 0, st, r);
+}
+
 hipError_t launch_rope(const RopeArgs & r, hipStream_t st) {
-    const uint32_t heads = (r.q ? r.a.nkv * r.gqa : 0) + 2 * r.a.nkv;
-    const dim3 grid((heads + 3) / 4, r.a.n);                         // n <= 65,535 (the host's launches)
-    if (r.a.hd == 128) hipLaunchKernelGGL(append_rope_kernel<128>, grid, dim3(256), 0, st, r);
-    else if (r.a.hd == 256) hipLaunchKernelGGL(append_rope_kernel<256>, grid, dim3(256), 0, st, r);
+    const uint32_t hpw = 512 / r.a.hd, nq = r.q ? r.a.nkv * r.gqa : 0;
+    // short chunks: an item per wave; long ones: all heads of a token in one workgroup, which shares its sines
+    const uint32_t all = ((nq + hpw - 1) / hpw + 2 * ((r.a.nkv + hpw - 1) / hpw) + 3) / 4, share = std::min(all, std::max(1u, 1024 / r.a.n));
+    const dim3 grid(share, r.a.n);                                   // n <= 65,535 (the host's launches)
+    if (r.a.hd == 128) launch_rope_hd<128>(r, grid, st);
+    else if (r.a.hd == 256) launch_rope_hd<256>(r, grid, st);
     else return hipErrorInvalidValue;
     return hipGetLastError();
 }
