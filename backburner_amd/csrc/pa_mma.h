@@ -65,6 +65,17 @@ __device__ __forceinline__ void mm_dequant(const MmRaw<FMT> & r, int half, pa_u4
     }
 }
 
+// e0, e1 rounded to fp16, and what the rounding left, e - fp16(e), rounded likewise: their sum keeps 22 bits. The difference by one
+// mixed-precision fma each (from the packed pair; as C++ it is a conversion there, one back and a subtraction)
+__device__ __forceinline__ void mm_split2(float e0, float e1, mm_h2 & hi, mm_h2 & lo) {
+    hi = (mm_h2){(_Float16) e0, (_Float16) e1};
+    const uint32_t u = __builtin_bit_cast(uint32_t, hi);
+    float r0, r1;
+    asm("v_fma_mix_f32 %0, -%1, 1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r0) : "v"(u), "v"(e0));
+    asm("v_fma_mix_f32 %0, -%1, 1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r1) : "v"(u), "v"(e1));
+    lo = (mm_h2){(_Float16) r0, (_Float16) r1};
+}
+
 __device__ __forceinline__ void mm_lds_barrier() {   // LDS-only workgroup barrier: loads in flight are not waited for
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
     __builtin_amdgcn_s_barrier();

@@ -490,11 +490,16 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void mma_kernel(const AttnArgs a) 
         if constexpr (PX) {
             float ts[2] = {0.0f, 0.0f};
             #pragma unroll
-            for (int v = 0; v < 16; v++) {
-                const float e = __builtin_amdgcn_exp2f(EX ? S[v] : fmaf(S[v], sm, -mref));
-                ts[v & 1] += e;
-                P[v / 8][v % 8] = (_Float16) e;
-                if constexpr (FMT != 0) Pl[v / 8][v % 8] = (_Float16) (e - (float) P[v / 8][v % 8]);
+            for (int v = 0; v < 16; v += 2) {
+                const float e0 = __builtin_amdgcn_exp2f(EX ? S[v] : fmaf(S[v], sm, -mref));
+                const float e1 = __builtin_amdgcn_exp2f(EX ? S[v + 1] : fmaf(S[v + 1], sm, -mref));
+                ts[0] += e0;
+                ts[1] += e1;
+                mm_h2 hi, lo;
+                if constexpr (FMT != 0) mm_split2(e0, e1, hi, lo);
+                else { hi = (mm_h2){(_Float16) e0, (_Float16) e1}; lo = hi; }
+                P[v / 8][v % 8] = hi[0]; P[v / 8][v % 8 + 1] = hi[1];
+                Pl[v / 8][v % 8] = lo[0]; Pl[v / 8][v % 8 + 1] = lo[1];
             }
             lsum += ts[0] + ts[1];
         } else {

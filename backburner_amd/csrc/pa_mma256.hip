@@ -328,11 +328,16 @@ __global__ __launch_bounds__(256, WPS) void mma256_kernel(const AttnArgs a) {
         if constexpr (PX) {
             float ts[2] = {0.0f, 0.0f};
             #pragma unroll
-            for (int v = 0; v < 8; v++) {
-                const float e = __builtin_amdgcn_exp2f(EX ? S[v / 4][v % 4] : fmaf(S[v / 4][v % 4], sm, -mref));
-                ts[v & 1] += e;
-                P[v] = (_Float16) e;
-                if constexpr (FMT != 0) Pl[v] = (_Float16) (e - (float) P[v]);
+            for (int v = 0; v < 8; v += 2) {
+                const float s0 = S[v / 4][v % 4], s1 = S[v / 4][v % 4 + 1];
+                const float e0 = __builtin_amdgcn_exp2f(EX ? s0 : fmaf(s0, sm, -mref)), e1 = __builtin_amdgcn_exp2f(EX ? s1 : fmaf(s1, sm, -mref));
+                ts[0] += e0;
+                ts[1] += e1;
+                mm_h2 hi, lo;
+                if constexpr (FMT != 0) mm_split2(e0, e1, hi, lo);
+                else { hi = (mm_h2){(_Float16) e0, (_Float16) e1}; lo = hi; }
+                P[v] = hi[0]; P[v + 1] = hi[1];
+                Pl[v] = lo[0]; Pl[v + 1] = lo[1];
             }
             lsum += ts[0] + ts[1];
         } else {
