@@ -821,7 +821,10 @@ extern "C" int pa_hip_attn_tree(pa_hip_ws * ws, const pa_hip_shape * s, const vo
         }
     if (left > 0) return bad("fewer keys than n_nodes");
     if (!ws) return bad("null workspace");
-    ta.mask = mask; ta.q = Q; ta.n_nodes = n_nodes; ta.hb = s->hb; ta.scale = s->scale;
+    ta.mask = mask; ta.q = Q; ta.n_nodes = n_nodes; ta.hb = s->hb; ta.rs = s->rs; ta.scale = s->scale;
+    ta.runs = 1; ta.cut = 64;
+    for (uint32_t j = 1; j < n_nodes; j++)
+        if (ta.k[j] != ta.k[j - 1] + s->rs || ta.v[j] != ta.v[j - 1] + s->rs) { ta.runs++; ta.cut = j; }
     Call cx;
     cx.ws = ws;
     cx.dec_groups = ws->dec_groups; cx.mma_workgroups = ws->mma_workgroups; cx.chunk_keys = ws->chunk_keys;

@@ -56,7 +56,8 @@ struct TreeArgs {
     const uint8_t * k[64], * v[64]; // key and value rows (head 0) of node j
     const uint64_t * mask;          // [n_nodes]
     const float * q;                // [nkv][rows][hd]
-    uint32_t n_nodes, hb;
+    uint32_t n_nodes, hb, rs;
+    uint32_t runs, cut;             // runs of nodes whose rows are rs apart; with two the second begins at node cut (1: 64)
     float scale;
 };
 hipError_t launch_tree(int hd, int fmt, const TreeArgs & a, hipStream_t st);

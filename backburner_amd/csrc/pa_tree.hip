@@ -9,48 +9,64 @@
 // matrix instruction multiplies a masked key's probability, zero, with whatever its value row holds, where infinities and NaN
 // become NaN. Here a value row that a row does not see is never read. At most 64 keys a row: vector work of a few instructions.
 //
-// W waves per row (1, 4 or 16 by the number of slots), each with every W-th slot and all of its loads issued at once, against its own
-// maximum; they meet once, through LDS. Lane l holds the dims (HD / 64) l .. of O. The first wave also takes the drafted keys, lane j
-// the score of key j (its key row read whole, the query's quants from LDS); only the ones that the row sees are touched, in a tree
-// the few on its path.
+// W waves per row (1, 2, 4 or 16 by the number of slots), each with every W-th slot and all of its loads issued at once, against its
+// own maximum; they meet once, through LDS. Lane l holds the dims (HD / 64) l .. of O. The row's first wave also takes the drafted
+// keys, only the ones that the row sees: four at a time, 16 lanes each, lane c with the dims (HD / 16) c .. of query, key and
+// value, so that a key's score is four lane swaps, and keys and values of 16 are in flight at once (a lane per key, whose row it reads
+// whole, and then a lane per dim took 5.0 us more of a call with 64 nodes of a tree, 24 of a chain).
 //
 #include "pa_attn.h"
 #include "pa_common.h"
 
 namespace pa_hip {
 
-template <int CTRL> __device__ __forceinline__ float tr_dpp(float v) {
-    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, false));
-}
-// max over the 8 or 16 lanes of a quant block (N lanes from a multiple of N on)
-template <int N> __device__ __forceinline__ float tr_blockmax(float v) {
-    v = fmaxf(v, tr_dpp<0xb1>(v));
-    v = fmaxf(v, tr_dpp<0x4e>(v));
-    v = fmaxf(v, tr_dpp<0x141>(v));                                  // row_half_mirror: lane ^ 7
-    if constexpr (N == 16) v = fmaxf(v, tr_dpp<0x140>(v));           // row_mirror: lane ^ 15
-    return v;
-}
-__device__ __forceinline__ float tr_wavemax(float v) {
-    #pragma unroll
-    for (int off = 32; off > 0; off >>= 1) v = fmaxf(v, __shfl_xor(v, off));
-    return v;
-}
+template <int CTRL> __device__ __forceinline__ int tr_dpp(int v) { return __builtin_amdgcn_update_dpp(0, v, CTRL, 0xf, 0xf, false); }
+template <int CTRL> __device__ __forceinline__ float tr_dpp(float v) { return __builtin_bit_cast(float, tr_dpp<CTRL>(__builtin_bit_cast(int, v))); }
 __device__ __forceinline__ float tr_wavesum(float v) {
     #pragma unroll
     for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off);
     return v;
 }
 
+// A lane's share of a head row, D = HD / 16 dims from dim D c on: whole bytes of its quant block (q8_0: D of the 32 values; q4_0: D bytes,
+// one nibble of each) and the block's scale, or D fp16 values
+template <int HD, int FMT> struct TrShare {
+    static constexpr int D = HD / 16, BB = FMT == 1 ? 34 : FMT == 2 ? 18 : 64, NW = FMT == 0 ? D / 2 : D / 4;
+    uint32_t w[NW];
+    float d;                                                         // the block's scale
+    __device__ __forceinline__ void zero() {
+        #pragma unroll
+        for (int i = 0; i < NW; i++) w[i] = 0u;
+        d = 0.0f;
+    }
+    __device__ __forceinline__ void load(const uint8_t * head, int c) {
+        if constexpr (FMT == 0) {
+            __builtin_memcpy(w, head + 2 * D * c, 2 * D);
+        } else {
+            const int b = c * D / 32, e = c * D % 32;
+            const uint8_t * p = head + BB * b;
+            d = pa_f16_bits_to_f32(pa_ld<uint16_t>(p));
+            __builtin_memcpy(w, p + 2 + (FMT == 1 ? e : e % 16), D);
+            if constexpr (FMT == 2) {
+                #pragma unroll
+                for (int i = 0; i < NW; i++) w[i] = (w[i] >> (e >= 16 ? 4 : 0)) & 0x0f0f0f0fu;   // element + 8
+            }
+        }
+    }
+    __device__ __forceinline__ float value(int k) const {            // without the scale
+        if constexpr (FMT == 0) return (float) pa_as_h2(w[k / 2])[k & 1];
+        else if constexpr (FMT == 1) return (float) (int8_t) (w[k / 4] >> (8 * (k % 4)));
+        else return (float) (int) ((w[k / 4] >> (8 * (k % 4))) & 0xffu) - 8.0f;
+    }
+};
+
 template <int HD, int FMT, int W> __global__ __launch_bounds__(W == 16 ? 1024 : 256) void tree_kernel(const TreeArgs a) {
-    constexpr int N = HD / 64, NBLK = HD / 32, BB = FMT == 1 ? 34 : FMT == 2 ? 18 : 64, NW = W == 16 ? 16 : 4, RPB = NW / W, S = 16;
-    // a row's query: int8 quants and block scales (quantized K), or fp16 values
-    __shared__ __attribute__((aligned(16))) uint32_t qs[RPB][HD / 2];
-    __shared__ float qd[RPB][NBLK], qsum[RPB][NBLK];
-    __shared__ float sm[W > 1 ? W : 1], sl[W > 1 ? W : 1];
-    __shared__ __attribute__((aligned(16))) float so[W > 1 ? W : 1][W > 1 ? HD : 1];
+    constexpr int N = HD / 64, D = HD / 16, NW = W == 16 ? 16 : 4, RPB = NW / W, S = 16, QL = 32 / D;   // QL lanes share a quant block
+    __shared__ float sm[NW], sl[NW];
+    __shared__ __attribute__((aligned(16))) float so[NW][HD];
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), wr = wave % W, rb = wave / W;
-    const uint32_t r = blockIdx.x * RPB + rb;                        // output row h * rows + i
-    if (r >= a.m.nkv * a.m.rows) return;                             // (W > 1: one row per workgroup, so none)
+    // (W = 1, 2: past the last row a wave repeats it, so that all meet at the barrier, and writes nothing)
+    const uint32_t rows = a.m.nkv * a.m.rows, r0 = blockIdx.x * RPB + rb, r = min(r0, rows - 1);   // output row h * rows + i
     const uint32_t h = r / a.m.rows, i = r % a.m.rows, nn = a.n_nodes, ns = a.m.n_slots;
     const size_t pr = ((size_t) h * a.m.qr + i) * a.m.rst;
 
@@ -78,110 +94,131 @@ template <int HD, int FMT, int W> __global__ __launch_bounds__(W == 16 ? 1024 : 
     #pragma unroll
     for (int k = 0; k < N; k++) acc[k] = 0.0f;
     if (wr == 0) {
-        const uint64_t sees = a.mask[i % nn] & (nn < 64 ? (1ull << nn) - 1 : ~0ull);
+        const int c = lane % 16, grp = lane / 16;
+        uint64_t left = a.mask[i % nn] & (nn < 64 ? (1ull << nn) - 1 : ~0ull);
         const size_t hoff = (size_t) h * a.hb;
-        // ---- the query, rounded as the attention kernels round it
+        // ---- the query, rounded as the attention kernels round it: this lane's dims as fp16 values, or as ggml's q8_0 quants with
+        // their block's scale times scale * log2 e and, for q4_0 keys, -8 * the sum of the block's quants
+        float x[D], qscale = a.scale * PA_LOG2E;
+        uint32_t qw[D / 4];
+        int q8 = 0;
+        __builtin_memcpy(x, a.q + (size_t) r * HD + D * c, 4 * D);
         {
             #pragma clang fp contract(off)
-            const float * q = a.q + (size_t) r * HD + N * lane;
-            float x[N];
-            #pragma unroll
-            for (int k = 0; k < N; k++) x[k] = q[k];
             if constexpr (FMT == 0) {
                 #pragma unroll
-                for (int k = 0; k < N; k += 2) {
-                    const pa_h2 v = {(_Float16) x[k], (_Float16) x[k + 1]};
-                    qs[rb][(N * lane + k) / 2] = pa_as_u32(v);
-                }
+                for (int k = 0; k < D; k++) x[k] = (float) (_Float16) x[k];
             } else {                                                 // quantize_row_q8_0_ref
                 float am = 0.0f;
                 #pragma unroll
-                for (int k = 0; k < N; k++) am = fmaxf(am, fabsf(x[k]));
-                am = tr_blockmax<32 / N>(am);
+                for (int k = 0; k < D; k++) am = fmaxf(am, fabsf(x[k]));
+                am = fmaxf(am, tr_dpp<0xb1>(am));
+                if constexpr (QL == 4) am = fmaxf(am, tr_dpp<0x4e>(am));
                 const float d = am / 127.0f, id = d != 0.0f ? 1.0f / d : 0.0f;
-                int s = 0;
                 #pragma unroll
-                for (int k = 0; k < N; k++) {
+                for (int k = 0; k < D / 4; k++) qw[k] = 0u;
+                #pragma unroll
+                for (int k = 0; k < D; k++) {
                     const int v = (int) roundf(x[k] * id);
-                    s += v;
-                    ((int8_t *) qs[rb])[N * lane + k] = (int8_t) v;
+                    q8 += v;
+                    qw[k / 4] |= ((uint32_t) v & 0xffu) << (8 * (k % 4));
+                }
+                q8 += tr_dpp<0xb1>(q8);
+                if constexpr (QL == 4) q8 += tr_dpp<0x4e>(q8);
+                q8 *= FMT == 2 ? -8 : 0;
+                qscale = (float) (_Float16) d * qscale;
+            }
+        }
+        // ---- group grp takes the row's visible keys grp, grp + 4, ..: a batch of B each at a time, all of its loads first
+        constexpr int B = HD == 128 ? 4 : 2;
+        #pragma unroll
+        for (int u = 0; u < 3; u++) left = u < grp ? left & (left - 1) : left;
+        float mg = -INFINITY, lg = 0.0f, og[D];
+        #pragma unroll
+        for (int k = 0; k < D; k++) og[k] = 0.0f;
+        while (__ballot(left != 0)) {
+            TrShare<HD, FMT> K[B], V[B];
+            bool is[B];
+            #pragma unroll
+            for (int u = 0; u < B; u++) {
+                is[u] = left != 0;
+                K[u].zero();
+                V[u].zero();
+                if (is[u]) {
+                    const uint32_t j = (uint32_t) __builtin_ctzll(left);
+                    // (the nodes mostly lie in one or two pages: their rows by arithmetic, otherwise from the table)
+                    const uint8_t * kr, * vr;
+                    if (a.runs <= 2) {
+                        const uint32_t run = j >= a.cut;
+                        kr = a.k[run ? a.cut : 0] + (size_t) (j - (run ? a.cut : 0)) * a.rs;
+                        vr = a.v[run ? a.cut : 0] + (size_t) (j - (run ? a.cut : 0)) * a.rs;
+                    } else {
+                        kr = a.k[j];
+                        vr = a.v[j];
+                    }
+                    K[u].load(kr + hoff, c);
+                    V[u].load(vr + hoff, c);
                 }
                 #pragma unroll
-                for (int off = 1; off < 32 / N; off <<= 1) s += __shfl_xor(s, off);
-                if (lane % (32 / N) == 0) { qd[rb][lane / (32 / N)] = (float) (_Float16) d; qsum[rb][lane / (32 / N)] = -8.0f * (float) s; }
+                for (int z = 0; z < 4; z++) left &= left - 1;        // (of 0 it is 0)
             }
-            __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");   // one wave's LDS operations run in order
-        }
-        // ---- lane j: the base-2 score of drafted key j
-        float s = -INFINITY;
-        if ((sees >> lane) & 1) {
-            const uint8_t * k = a.k[lane] + hoff;
-            float t = 0.0f;
+            float s[B], mb = mg;
             #pragma unroll
-            for (int b = 0; b < NBLK; b++) {
+            for (int u = 0; u < B; u++) {
+                float t = 0.0f;
                 if constexpr (FMT == 0) {
                     #pragma unroll
-                    for (int c = 0; c < 4; c++) {
-                        const pa_u4 kw = pa_ld<pa_u4>(k + 64 * b + 16 * c), qw = *(const pa_u4 *) &qs[rb][16 * b + 4 * c];
-                        #pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            const pa_h2 kv = pa_as_h2(kw[e]), qv = pa_as_h2(qw[e]);
-                            t = fmaf((float) kv[0], (float) qv[0], t);
-                            t = fmaf((float) kv[1], (float) qv[1], t);
-                        }
-                    }
+                    for (int k = 0; k < D; k++) t = fmaf(K[u].value(k), x[k], t);
+                    t += tr_dpp<0xb1>(t);
+                    t += tr_dpp<0x4e>(t);
                 } else {
-                    const float d = pa_f16_bits_to_f32(pa_ld<uint16_t>(k + BB * b));
-                    const pa_u4 q0 = *(const pa_u4 *) &qs[rb][8 * b], q1 = *(const pa_u4 *) &qs[rb][8 * b + 4];
-                    const pa_u4 k0 = pa_ld<pa_u4>(k + BB * b + 2);
-                    pa_u4 w0 = k0, w1;
-                    if constexpr (FMT == 1) w1 = pa_ld<pa_u4>(k + BB * b + 18);
-                    else { w0 = k0 & 0x0f0f0f0fu; w1 = (k0 >> 4) & 0x0f0f0f0fu; }   // nibbles as they are: element + 8
                     int dot = 0;
                     #pragma unroll
-                    for (int c = 0; c < 4; c++) {
-                        dot = __builtin_amdgcn_sdot4((int) w0[c], (int) q0[c], dot, false);
-                        dot = __builtin_amdgcn_sdot4((int) w1[c], (int) q1[c], dot, false);
-                    }
-                    t = fmaf(((float) dot + (FMT == 2 ? qsum[rb][b] : 0.0f)) * qd[rb][b], d, t);
+                    for (int k = 0; k < D / 4; k++) dot = __builtin_amdgcn_sdot4((int) K[u].w[k], (int) qw[k], dot, false);
+                    dot += tr_dpp<0xb1>(dot);
+                    if constexpr (QL == 4) dot += tr_dpp<0x4e>(dot);
+                    t = (float) (dot + q8) * K[u].d;                 // the whole block's dot in each of its lanes
                 }
+                // over the lanes of the other blocks: 7 - c, 15 - c (at two lanes a block c ^ 2 too)
+                t *= qscale;
+                if constexpr (FMT != 0 && QL == 2) t += tr_dpp<0x4e>(t);
+                t += tr_dpp<0x141>(t);
+                t += tr_dpp<0x140>(t);
+                s[u] = is[u] ? t : -INFINITY;
+                mb = fmaxf(mb, s[u]);
             }
-            s = t * (a.scale * PA_LOG2E);
-        }
-        m = tr_wavemax(s);
-        const float p = __builtin_amdgcn_exp2f(s - (m == -INFINITY ? 0.0f : m));
-        L = p;
-        // ---- the drafted values, four at a time: lane l's dims N l .. of each key the row sees
-        const int d0 = N * lane, b = d0 / 32, e = d0 % 32;
-        for (uint64_t left = sees; left;) {
-            float x[4][N], pj[4];
+            const float ms = mb == -INFINITY ? 0.0f : mb, f = __builtin_amdgcn_exp2f((mg == -INFINITY ? ms : mg) - ms);
+            lg *= f;
             #pragma unroll
-            for (int u = 0; u < 4; u++) {
-                const bool is = left != 0;                           // uniform
-                const int j = is ? __builtin_ctzll(left) : 0;
-                left &= left - 1;
-                pj[u] = is ? __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, p), j)) : 0.0f;
+            for (int k = 0; k < D; k++) og[k] *= f;
+            #pragma unroll
+            for (int u = 0; u < B; u++) {
+                const float p = __builtin_amdgcn_exp2f(s[u] - ms), pd = FMT == 0 ? p : p * V[u].d;
+                lg += p;
                 #pragma unroll
-                for (int k = 0; k < N; k++) x[u][k] = 0.0f;
-                if (!is) continue;
-                const uint8_t * v = a.v[j] + hoff;
-                if constexpr (FMT == 0) {
-                    #pragma unroll
-                    for (int k = 0; k < N; k++) x[u][k] = pa_f16_bits_to_f32(pa_ld<uint16_t>(v + 2 * (d0 + k)));
-                } else {
-                    const float d = pa_f16_bits_to_f32(pa_ld<uint16_t>(v + BB * b));
-                    #pragma unroll
-                    for (int k = 0; k < N; k++) {
-                        if constexpr (FMT == 1) x[u][k] = d * (float) (int8_t) v[BB * b + 2 + e + k];
-                        else x[u][k] = d * (float) ((int) ((v[BB * b + 2 + (e & 15) + k] >> (e & 16 ? 4 : 0)) & 15) - 8);
-                    }
-                }
+                for (int k = 0; k < D; k++) og[k] = fmaf(pd, V[u].value(k), og[k]);
             }
-            #pragma unroll
-            for (int u = 0; u < 4; u++)
-                #pragma unroll
-                for (int k = 0; k < N; k++) acc[k] = fmaf(pj[u], x[u][k], acc[k]);
+            mg = mb;
         }
+        // ---- the four groups, then from 16 lanes' dims to 64
+        m = fmaxf(mg, __shfl_xor(mg, 16));
+        m = fmaxf(m, __shfl_xor(m, 32));
+        const float ms = m == -INFINITY ? 0.0f : m, f = __builtin_amdgcn_exp2f((mg == -INFINITY ? ms : mg) - ms);
+        lg *= f;
+        L = c == 0 ? lg : 0.0f;                                      // (summed over the wave below)
+        #pragma unroll
+        for (int k = 0; k < D; k++) {
+            og[k] *= f;
+            og[k] += __shfl_xor(og[k], 16);
+            og[k] += __shfl_xor(og[k], 32);
+        }
+        if (grp == 0)
+            #pragma unroll
+            for (int k = 0; k < D; k++) so[wave][D * c + k] = og[k];
+        __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");       // one wave's LDS operations run in order
+        #pragma unroll
+        for (int k = 0; k < N; k++) acc[k] = so[wave][N * lane + k];
+        __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
     }
 
     // ---- the slots
@@ -210,14 +247,14 @@ template <int HD, int FMT, int W> __global__ __launch_bounds__(W == 16 ? 1024 : 
 
     // ---- the row's waves
     if constexpr (W > 1) {
-        if (lane == 0) { sm[wr] = m; sl[wr] = L; }
+        if (lane == 0) { sm[wave] = m; sl[wave] = L; }
         #pragma unroll
-        for (int k = 0; k < N; k++) so[wr][N * lane + k] = acc[k];
+        for (int k = 0; k < N; k++) so[wave][N * lane + k] = acc[k];
         __syncthreads();
         if (wr != 0) return;
-        float M = sm[0];
+        float M = sm[wave];
         #pragma unroll
-        for (int u = 1; u < W; u++) M = fmaxf(M, sm[u]);
+        for (int u = 1; u < W; u++) M = fmaxf(M, sm[wave + u]);
         const float Ms = M == -INFINITY ? 0.0f : M;
         float f = __builtin_amdgcn_exp2f((m == -INFINITY ? Ms : m) - Ms);   // (a NaN of the drafted keys stays in acc and L)
         L *= f;
@@ -225,13 +262,14 @@ template <int HD, int FMT, int W> __global__ __launch_bounds__(W == 16 ? 1024 : 
         for (int k = 0; k < N; k++) acc[k] *= f;
         #pragma unroll
         for (int u = 1; u < W; u++) {
-            f = __builtin_amdgcn_exp2f(sm[u] - Ms);
-            L = fmaf(f, sl[u], L);
+            f = __builtin_amdgcn_exp2f(sm[wave + u] - Ms);
+            L = fmaf(f, sl[wave + u], L);
             #pragma unroll
-            for (int k = 0; k < N; k++) acc[k] = fmaf(f, so[u][N * lane + k], acc[k]);
+            for (int k = 0; k < N; k++) acc[k] = fmaf(f, so[wave + u][N * lane + k], acc[k]);
         }
         m = M;
     }
+    if (r0 >= rows) return;
 
     // ---- the reply format
     const float inv = L == 0.0f ? 0.0f : 1.0f / L;
@@ -244,6 +282,7 @@ template <int HD, int FMT, int W> __global__ __launch_bounds__(W == 16 ? 1024 : 
 template <int HD, int FMT> static void launch_tree_w(const TreeArgs & a, hipStream_t st) {
     const uint32_t rows = a.m.nkv * a.m.rows;
     if (a.m.n_slots <= 16) hipLaunchKernelGGL((tree_kernel<HD, FMT, 1>), dim3((rows + 3) / 4), dim3(256), 0, st, a);
+    else if (a.m.n_slots <= 32) hipLaunchKernelGGL((tree_kernel<HD, FMT, 2>), dim3((rows + 1) / 2), dim3(256), 0, st, a);
     else if (a.m.n_slots <= 64) hipLaunchKernelGGL((tree_kernel<HD, FMT, 4>), dim3(rows), dim3(256), 0, st, a);
     else hipLaunchKernelGGL((tree_kernel<HD, FMT, 16>), dim3(rows), dim3(1024), 0, st, a);
 }
