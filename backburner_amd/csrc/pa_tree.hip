@@ -9,7 +9,7 @@
 // matrix instruction multiplies a masked key's probability, zero, with whatever its value row holds, where infinities and NaN
 // become NaN. Here a value row that a row does not see is never read. At most 64 keys a row: vector work of a few instructions.
 //
-// W waves per row (1, 2, 4 or 16 by the number of slots), each with every W-th slot and all of its loads issued at once, against its
+// W waves per row (1, 2, 4 or 8 by the number of slots), each with every W-th slot and all of its loads issued at once, against its
 // own maximum; they meet once, through LDS. Lane l holds the dims (HD / 64) l .. of O. The row's first wave also takes the drafted
 // keys, only the ones that the row sees: four at a time, 16 lanes each, lane c with the dims (HD / 16) c .. of query, key and
 // value, so that a key's score is four lane swaps, and keys and values of 16 are in flight at once (a lane per key, whose row it reads
@@ -60,8 +60,8 @@ template <int HD, int FMT> struct TrShare {
     }
 };
 
-template <int HD, int FMT, int W> __global__ __launch_bounds__(W == 16 ? 1024 : 256) void tree_kernel(const TreeArgs a) {
-    constexpr int N = HD / 64, D = HD / 16, NW = W == 16 ? 16 : 4, RPB = NW / W, S = 16, QL = 32 / D;   // QL lanes share a quant block
+template <int HD, int FMT, int W> __global__ __launch_bounds__(W == 8 ? 512 : 256) void tree_kernel(const TreeArgs a) {
+    constexpr int N = HD / 64, D = HD / 16, NW = W == 8 ? 8 : 4, RPB = NW / W, S = 16, QL = 32 / D;   // QL lanes share a quant block
     __shared__ float sm[NW], sl[NW];
     __shared__ __attribute__((aligned(16))) float so[NW][HD];
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), wr = wave % W, rb = wave / W;
@@ -284,7 +284,7 @@ template <int HD, int FMT> static void launch_tree_w(const TreeArgs & a, hipStre
     if (a.m.n_slots <= 16) hipLaunchKernelGGL((tree_kernel<HD, FMT, 1>), dim3((rows + 3) / 4), dim3(256), 0, st, a);
     else if (a.m.n_slots <= 32) hipLaunchKernelGGL((tree_kernel<HD, FMT, 2>), dim3((rows + 1) / 2), dim3(256), 0, st, a);
     else if (a.m.n_slots <= 64) hipLaunchKernelGGL((tree_kernel<HD, FMT, 4>), dim3(rows), dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((tree_kernel<HD, FMT, 16>), dim3(rows), dim3(1024), 0, st, a);
+    else hipLaunchKernelGGL((tree_kernel<HD, FMT, 8>), dim3(rows), dim3(512), 0, st, a);
 }
 
 template <int HD> static hipError_t launch_tree_hd(int fmt, const TreeArgs & a, hipStream_t st) {
