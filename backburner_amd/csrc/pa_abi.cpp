@@ -13,6 +13,7 @@
 #include <cstdlib>
 #include <cstring>
 #include <mutex>
+#include <new>
 #include <string>
 #include <thread>
 #include <vector>
@@ -808,7 +809,8 @@ extern "C" int pa_hip_attn_tree(pa_hip_ws * ws, const pa_hip_shape * s, const vo
         return bad("mask and Oh must be 8-byte, Q and lse 4-byte aligned");
     // the last n_nodes keys, from the last page back; what is left is the context
     static thread_local std::vector<uint32_t> context;
-    context.assign(nkeys, nkeys + n_pages);
+    try { context.assign(nkeys, nkeys + n_pages); }
+    catch (const std::bad_alloc &) { return bad("out of host memory"); }
     TreeArgs ta;
     std::memset(&ta, 0, sizeof ta);
     uint32_t left = n_nodes;
@@ -1054,30 +1056,38 @@ extern "C" int pa_hip_copy_rows(const pa_hip_shape * s, int n_layers, const void
     if (dlast >= (uint64_t) dst_pages * page_keys) return bad("destination positions past the last page");
     const uint32_t sp0 = (uint32_t) (first / page_keys), sp1 = (uint32_t) (last / page_keys);
     const uint32_t dp0 = dst_pos0 / page_keys, dp1 = (uint32_t) (dlast / page_keys);
-    // every touched page, to see which are both: (pointer, place of the table), destinations first
+    // every touched page, to see which are both: destinations by pointer in a table of open addressing, then the sources against it
     bool in_place = false;
     {
-        static thread_local std::vector<std::pair<uintptr_t, uint64_t>> dst;
-        dst.clear();
+        struct Page { const void * p; uint64_t place; };
+        static thread_local std::vector<Page> table;
+        size_t size = 64;
+        while (size < 2 * (size_t) n_layers * 2 * (dp1 - dp0 + 1)) size *= 2;
+        try { table.assign(size, Page{nullptr, 0}); }
+        catch (const std::bad_alloc &) { return bad("out of host memory"); }
+        auto find = [&](const void * x) -> Page & {
+            size_t k = ((uintptr_t) x >> 8) * 0x9e3779b97f4a7c15ull >> 20;
+            while (table[k &= size - 1].p && table[k].p != x) k++;
+            return table[k];
+        };
         auto place = [&](int layer, int tensor, uint32_t p) { return ((uint64_t) layer * 2 + tensor) << 32 | p; };
         for (int l = 0; l < n_layers; l++)
             for (int t = 0; t < 2; t++)
                 for (uint32_t p = dp0; p <= dp1; p++) {
                     const void * x = (t ? dst_v : dst_k)[(size_t) l * dst_pages + p];
                     if (!x) return bad("null destination page " + std::to_string(p) + " of layer " + std::to_string(l));
-                    dst.push_back({(uintptr_t) x, place(l, t, p)});
+                    Page & at = find(x);
+                    if (at.p) return bad("a page is a destination twice");
+                    at = Page{x, place(l, t, p)};
                 }
-        std::sort(dst.begin(), dst.end());
-        for (size_t i = 1; i < dst.size(); i++)
-            if (dst[i].first == dst[i - 1].first) return bad("a page is a destination twice");
         for (int l = 0; l < n_layers; l++)
             for (int t = 0; t < 2; t++)
                 for (uint32_t p = sp0; p <= sp1; p++) {
                     const void * x = (t ? src_v : src_k)[(size_t) l * src_pages + p];
                     if (!x) return bad("null source page " + std::to_string(p) + " of layer " + std::to_string(l));
-                    const auto at = std::lower_bound(dst.begin(), dst.end(), std::make_pair((uintptr_t) x, (uint64_t) 0));
-                    if (at == dst.end() || at->first != (uintptr_t) x) continue;
-                    if (at->second != place(l, t, p)) return bad("a page is a source and, at another place, a destination");
+                    const Page & at = find(x);
+                    if (!at.p) continue;
+                    if (at.place != place(l, t, p)) return bad("a page is a source and, at another place, a destination");
                     in_place = true;
                 }
     }
