@@ -136,7 +136,7 @@ __device__ __forceinline__ int lp_above(lp_key mine, lp_key * best) {
     best[threadIdx.x % 64] = mine;
     lp_wave_sync();
     int above = 0;
-    #pragma unroll 4
+    #pragma unroll 8
     for (int i = 0; i < 64; i += 2) {
         const pa_u4 x = *(const pa_u4 *) (best + i);
         above += (((lp_key) x.y << 32) | x.x) > mine;
@@ -151,7 +151,7 @@ __device__ __forceinline__ uint32_t lp_nth_value(int n, uint32_t mine, lp_key * 
     b[threadIdx.x % 64] = mine;
     lp_wave_sync();
     int above = 0;
-    #pragma unroll 4
+    #pragma unroll 8
     for (int i = 0; i < 64; i += 4) {
         const pa_u4 x = *(const pa_u4 *) (b + i);
         above += (x.x > mine) + (x.y > mine) + (x.z > mine) + (x.w > mine);
@@ -240,8 +240,13 @@ __device__ __forceinline__ void lp_rank(LpTop & l, LpShared & sh) {
         const lp_key k = sh.tops[w][i];
         int place = 0;
         #pragma unroll 2
-        for (int j = 0; j < l.n; j++)
-            place += (sh.tops[0][j] > k) + (sh.tops[1][j] > k) + (sh.tops[2][j] > k) + (sh.tops[3][j] > k);
+        for (int j = 0; j < l.n; j += 2)                             // (past a wave's best there are zeros)
+            #pragma unroll
+            for (int o = 0; o < 4; o++) {
+                const pa_u4 x = *(const pa_u4 *) &sh.tops[o][j];
+                place += (((lp_key) x.y << 32) | x.x) > k;
+                place += (((lp_key) x.w << 32) | x.z) > k;
+            }
         if (k && place < l.n) sh.out[place] = k;
     }
     __syncthreads();
@@ -254,6 +259,15 @@ template <typename T> __global__ __launch_bounds__(256) void logprob_kernel(cons
     const T * x = (const T *) a.logits + (size_t) row * (size_t) a.stride;
     const uint32_t j0 = (uint32_t) w * a.span, j1 = (uint32_t) min((int64_t) a.vocab, (int64_t) j0 + a.span);
     const float c2 = a.scale * PA_LOG2E;
+    // the first 256 given ids' logits, on their way while the row is joined
+    int32_t id = -1;
+    float given = 0.0f;
+    auto given_load = [&] {
+        if (t >= a.n_given) return;
+        id = a.given[(size_t) row * a.n_given + t];
+        if (id >= 0 && id < a.vocab) given = L::value(x[id]);
+    };
+    if (a.parts == 1) given_load();
     LpPart p = {-INFINITY, 0.0f, 0.0f};
     extern __shared__ __attribute__((aligned(16))) lp_key lists[];   // [4][lp_room(n_top)], then [4][LP_NV / 4][64] x 4 floats
     pa_f4 * vals = (pa_f4 *) (lists + 4 * lp_room(a.n_top)) + 64 * (LP_NV / 4) * (t / 64) + t % 64;
@@ -306,25 +320,29 @@ template <typename T> __global__ __launch_bounds__(256) void logprob_kernel(cons
         #pragma unroll
         for (int u = 0; u < LP_NV / 4; u++) vals[64 * u] = (pa_f4){v[4 * u], v[4 * u + 1], v[4 * u + 2], v[4 * u + 3]};
         lp_wave_sync();
-        while (__ballot(left != 0)) {
+        for (;;) {
+            const bool more = __ballot(left != 0) != 0;
+            // sorted where the list might not take another 64, and after the segment for a new floor
+            if (more ? top.count + 64 > lp_room(top.n)
+                     : j + LP_SEG < j1 && top.count >= (top.floor == 0 ? top.n : top.n + LP_MORE)) {
+                top.sort();
+                if (t % 64 == 0) sh.fval[t / 64] = top.fval;
+            }
+            if (!more) break;
             const uint32_t i = __builtin_ctz(left | 1u << 31) & (LP_NV - 1);
             const float val = ((const float *) (vals + 64 * (i / 4)))[i % 4];
             const uint32_t at = L::at(i, t);
             const lp_key k = left != 0 && at < n ? lp_make_key(val, j + at) : 0;
             left &= left - 1;
-            if (top.count + 64 > lp_room(top.n)) top.sort();
             top.push(k > top.floor, k);
         }
-        if (j + LP_SEG < j1 && top.count >= (top.floor == 0 ? top.n : top.n + LP_MORE)) {
-            top.sort();
-            if (t % 64 == 0) sh.fval[t / 64] = top.fval;
-        }
     }
-    if (a.n_top > 0) lp_rank(top, sh);
-    p = lp_join_all(p, c2, sh.red);
-
-    if (a.parts > 1) {
-        // this workgroup's part and best keys, written through and complete before it counts itself done
+    // this part, then, by the row's last workgroup, all of them (one code for both: it runs once, and is fetched once)
+    for (bool joined = a.parts == 1;; joined = true) {
+        if (a.n_top > 0) lp_rank(top, sh);
+        p = lp_join_all(p, c2, sh.red);
+        if (joined) break;
+        // the part and its best keys, written through and complete before the workgroup counts itself done
         float2 * part = (float2 *) a.part + 2 * ((size_t) row * a.parts + w);
         lp_key * keys = a.keys + ((size_t) row * a.parts + w) * a.n_top;
         if (t < a.n_top) __hip_atomic_store(&keys[t], sh.out[t], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -340,6 +358,7 @@ template <typename T> __global__ __launch_bounds__(256) void logprob_kernel(cons
         }
         __syncthreads();
         if (!sh.last) return;
+        given_load();
         part = (float2 *) a.part + 2 * (size_t) row * a.parts;
         keys = a.keys + (size_t) row * a.parts * a.n_top;
         p = LpPart{-INFINITY, 0.0f, 0.0f};
@@ -355,8 +374,6 @@ template <typename T> __global__ __launch_bounds__(256) void logprob_kernel(cons
             const lp_key k = i < nk ? __hip_atomic_load(&keys[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0;
             top.push(k != 0, k);
         }
-        p = lp_join_all(p, c2, sh.red);
-        if (a.n_top > 0) lp_rank(top, sh);
     }
 
     const bool bad = p.s != p.s || p.m == INFINITY, none = p.m == -INFINITY;
@@ -366,9 +383,10 @@ template <typename T> __global__ __launch_bounds__(256) void logprob_kernel(cons
         if (a.lse) a.lse[row] = bad ? NAN : none ? -INFINITY : fmaf(p.m, a.scale, ls);
         if (a.entropy) a.entropy[row] = bad ? NAN : none ? 0.0f : ls - a.scale * p.t / p.s;
     }
-    for (int i = t; i < a.n_given; i += 256) {
-        const int32_t id = a.given[(size_t) row * a.n_given + i];
-        a.logp[(size_t) row * a.n_given + i] = id >= 0 && id < a.vocab ? logp_of(L::value(x[id])) : NAN;
+    if (t < a.n_given) a.logp[(size_t) row * a.n_given + t] = id >= 0 && id < a.vocab ? logp_of(given) : NAN;
+    for (int i = t + 256; i < a.n_given; i += 256) {
+        const int32_t j = a.given[(size_t) row * a.n_given + i];
+        a.logp[(size_t) row * a.n_given + i] = j >= 0 && j < a.vocab ? logp_of(L::value(x[j])) : NAN;
     }
     if (t < a.n_top) {
         const lp_key k = sh.out[t];
