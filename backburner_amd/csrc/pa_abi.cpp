@@ -792,6 +792,13 @@ extern "C" int pa_hip_coattn_merge(const uint16_t * Oh, const float * lse, const
                   "coattn launch") ? 0 : -1;
 }
 
+namespace {
+bool on_device(const pa_hip_ws * ws) {
+    int dev = -1;
+    return hipGetDevice(&dev) == hipSuccess && dev == ws->device;
+}
+}  // namespace
+
 // The context goes through the attention kernels, whose slots (never a direct result) the tree kernel joins with the drafted
 // keys: their rows' addresses travel in its arguments, so they may lie in any pages.
 extern "C" int pa_hip_attn_tree(pa_hip_ws * ws, const pa_hip_shape * s, const void * const * k_pages, const void * const * v_pages,
@@ -823,6 +830,7 @@ extern "C" int pa_hip_attn_tree(pa_hip_ws * ws, const pa_hip_shape * s, const vo
         }
     if (left > 0) return bad("fewer keys than n_nodes");
     if (!ws) return bad("null workspace");
+    if (!on_device(ws)) return bad("the workspace belongs to another device than the current one");
     ta.mask = mask; ta.q = Q; ta.n_nodes = n_nodes; ta.hb = s->hb; ta.rs = s->rs; ta.scale = s->scale;
     ta.runs = 1; ta.cut = 64;
     for (uint32_t j = 1; j < n_nodes; j++)
@@ -844,7 +852,7 @@ extern "C" int pa_hip_logprobs(pa_hip_ws * ws, const void * logits, int type, in
     if (n_rows < 0 || n_rows > (1 << 20)) return bad("n_rows must be 0..2^20");
     if (vocab < 1 || vocab > (1 << 24)) return bad("vocab must be 1..2^24");
     if (row_stride < vocab || row_stride > (1ll << 40)) return bad("row_stride must be vocab..2^40");
-    if (!(scale > 0.0f) || !std::isfinite(scale)) return bad("scale must be finite and > 0");
+    if (!(scale >= 0x1p-64f && scale <= 0x1p64f)) return bad("scale must be 2^-64..2^64");
     if (n_given < 0 || n_given > 1024 || n_top < 0 || n_top > 32) return bad("n_given must be 0..1024 and n_top 0..32");
     if (n_rows == 0) return 0;
     if (!logits || (n_given > 0 && (!given || !logp)) || (n_top > 0 && (!top_id || !top_logp))) return bad("null argument");
@@ -852,6 +860,7 @@ extern "C" int pa_hip_logprobs(pa_hip_ws * ws, const void * logits, int type, in
         !aligned(top_id, 4) || !aligned(top_logp, 4))
         return bad("logits must be aligned to their type, the other arrays to 4 bytes");
     if (!ws) return bad("null workspace");
+    if (!on_device(ws)) return bad("the workspace belongs to another device than the current one");
     LogprobArgs a;
     const int64_t segs = (vocab + 4095) / 4096;
     // Workgroups of a row: 1,024 in all, four per CU (what is resident at once); more only add ends, fewer leave loads unhidden. us at

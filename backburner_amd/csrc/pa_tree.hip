@@ -149,9 +149,9 @@ template <int HD, int FMT, int W> __global__ __launch_bounds__(W == 8 ? 512 : 25
                     // (the nodes mostly lie in one or two pages: their rows by arithmetic, otherwise from the table)
                     const uint8_t * kr, * vr;
                     if (a.runs <= 2) {
-                        const uint32_t run = j >= a.cut;
-                        kr = a.k[run ? a.cut : 0] + (size_t) (j - (run ? a.cut : 0)) * a.rs;
-                        vr = a.v[run ? a.cut : 0] + (size_t) (j - (run ? a.cut : 0)) * a.rs;
+                        const uint32_t first = j >= a.cut ? a.cut % 64 : 0;   // (one run: cut is 64, never reached)
+                        kr = a.k[first] + (size_t) (j - first) * a.rs;
+                        vr = a.v[first] + (size_t) (j - first) * a.rs;
                     } else {
                         kr = a.k[j];
                         vr = a.v[j];

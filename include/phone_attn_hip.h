@@ -185,7 +185,7 @@ int pa_hip_coattn_merge(const uint16_t * Oh, const float * lse, const float * O_
  * the call runs, so that a captured call replays with the tree that is there then; bits from n_nodes on are ignored. What a
  * row does not see never enters its result, whatever the bytes there (infinities, NaN). The reply format: Oh = f16(O / l)
  * (fp16 bits [nkv][rows][hd], 8-byte aligned; 0 for a row that sees no key), lse = m + log l (fp32 [nkv][rows]; -inf there).
- * PA_QMODE_GGML only. Returns 0 once enqueued, -1 on a bad argument (nothing enqueued). */
+ * PA_QMODE_GGML only; scale * |Q| below 90,000. Returns 0 once enqueued, -1 on a bad argument (nothing enqueued). */
 int pa_hip_attn_tree(pa_hip_ws * ws, const pa_hip_shape * shape, const void * const * k_pages, const void * const * v_pages,
                      const uint32_t * nkeys, int n_pages, uint32_t n_nodes, const uint64_t * mask, const float * Q,
                      uint16_t * Oh, float * lse, void * stream);
@@ -194,8 +194,9 @@ int pa_hip_attn_tree(pa_hip_ws * ws, const pa_hip_shape * shape, const void * co
 enum { PA_TYPE_F32 = 0, PA_TYPE_F16 = 1, PA_TYPE_BF16 = 2 };
 
 /* What sampled acceptance and scoring read off the logits, beside pa_hip_accept's argmax (no counterpart in the reference):
- * row i of n_rows (0 .. 2^20) starts at element i*row_stride (>= vocab) of `logits` (type PA_TYPE_*, aligned to its size), and with
- * y = scale * logits (scale > 0: 1 / temperature)
+ * row i of n_rows (0 .. 2^20) starts at element i*row_stride (>= vocab, which is 1 .. 2^24) of `logits` (type PA_TYPE_*,
+ * aligned to its size), and with
+ * y = scale * logits (scale: 1 / temperature, 2^-64 .. 2^64)
  *   lse[i]          = log sum_j e^y_j
  *   logp[i][g]      = y[given[i][g]] - lse[i], g < n_given (0 .. 1024); NaN for an id outside 0 .. vocab-1
  *   entropy[i]      = -sum_j p_j log p_j, p_j = e^(y_j - lse[i])

@@ -193,6 +193,48 @@ def test_tree_own_stream_repeats(ws):
     check_tree(shape, K, V, 3000, Q, 20, mask, a)
 
 
+def test_tree_offsets_past_32_bits(ws):
+    """One page of rows 32 MB apart, 6.7 GB of it: the context's and the tree's rows lie past 32 bits of offset; a rope append
+    writes there, and a copy moves rows there."""
+    nkv, gqa, hd, nodes, n, rs = 2, 4, 128, 9, 200, 1 << 25
+    rng, small, K, V, Q = tree_case(33, Q8, nkv, gqa, hd, nodes, n)
+    shape = bb.make_shape(nkv, gqa * nodes, hd, Q8, rs=rs)
+    _, mask = plain.random_tree(rng, nodes)
+    k, v = bb.DeviceBuffer((n - 1) * rs + small.rs), bb.DeviceBuffer((n - 1) * rs + small.rs)
+    dq, dm = buf(Q), buf(mask)
+    do, dl = bb.DeviceBuffer(nkv * gqa * nodes * hd * 2), bb.DeviceBuffer(nkv * gqa * nodes * 4)
+    put = lambda b, rows, j: b.upload(rows[j * small.rs:(j + 1) * small.rs], j * rs)  # noqa: E731
+    get = lambda b, j: b.download(np.uint8, small.rs, j * rs)  # noqa: E731
+    try:
+        print("tree past 32 bits", flush=True)
+        for j in range(n):
+            put(k, K, j); put(v, V, j)
+        pages = bb.Pages([k.ptr], [v.ptr], [n], [])
+        ws.attn_tree(shape, pages, nodes, dm.ptr, dq.ptr, do.ptr, dl.ptr)
+        bb.device_sync()
+        got = (do.download(np.uint16).reshape(-1, hd), dl.download(np.float32))
+        check_tree(small, K, V, n, Q, nodes, mask, got)
+        table = bb.LayerTable([pages])
+        bb.copy_rows(shape, table, table, n, [191, 193, 198], 191)
+        bb.device_sync()
+        for X, b in ((K, k), (V, v)):
+            for at, j in ((191, 191), (192, 193), (193, 198), (194, 194), (199, 199)):
+                assert np.array_equal(get(b, at), X[j * small.rs:(j + 1) * small.rs])
+        x = rng.standard_normal((2, 2 * nkv * hd)).astype(np.float32)
+        dx, dp = buf(x), buf(np.arange(2, dtype=np.int32))
+        rope = bb.make_rope(None, None, 0.0, None, 0, k_stride=2 * nkv * hd, v_stride=2 * nkv * hd)
+        bb.append_rope(bb.make_shape(nkv, 0, hd, Q8, rs=rs), pages, n, 197, rope, None, dx.ptr, dx.ptr + 4 * nkv * hd, dp.ptr, 2, None)
+        bb.device_sync()
+        for t, b in ((0, k), (1, v)):
+            vals = np.ascontiguousarray(x.reshape(2, 2, nkv, hd)[:, t])
+            want = orc.rows_from_f32(Q8, vals, small.rs, small.hb)
+            assert np.array_equal(np.concatenate([get(b, 197), get(b, 198)]), want)
+        dx.close(); dp.close()
+    finally:
+        for b in (k, v, dq, dm, do, dl):
+            b.close()
+
+
 # ---------------------------------------------------------------- norm, rotation and append
 def to_type(x, type):
     """fp32 as the bytes of `type`, and the values these hold."""
@@ -375,6 +417,39 @@ def test_logprobs_edges(ws, vocab):
         check_logprobs(x, 1.0, given, n_top, gpu_logprobs(ws, x, bb.TYPE_F32, vocab, 1.0, given, n_top))
 
 
+def test_logprobs_best_in_few_places(ws):
+    """The best in every other 4,096 values only (the join's lists then hold them in half of the lanes), all in one thread's share,
+    and in ascending and descending runs of the whole row."""
+    rng = np.random.default_rng(5)
+    vocab = 38 * 4096 - 7
+    x = rng.standard_normal((4, vocab)).astype(np.float32)
+    x[0] += np.where(np.arange(vocab) // 4096 % 2 == 0, 100.0, 0.0).astype(np.float32)
+    x[1, 20::1024] += 50.0
+    x[2] = np.sort(x[2])
+    x[3] = np.sort(x[3])[::-1]
+    given = rng.integers(0, vocab, (4, 1)).astype(np.int32)
+    print("logprobs few places", flush=True)
+    for rows in ([0], [1], [2], [3], [0, 1, 2, 3]):
+        for n_top in (32, 31, 3):
+            check_logprobs(x[rows], 1.0, given[rows], n_top, gpu_logprobs(ws, x[rows], bb.TYPE_F32, vocab, 1.0, given[rows], n_top))
+
+
+def test_logprobs_largest_vocabulary(ws):
+    vocab = 1 << 24
+    rng = np.random.default_rng(6)
+    x = rng.standard_normal((1, vocab)).astype(np.float32)
+    best = rng.choice(vocab, 32, replace=False)
+    x[0, best] = 10.0 + np.arange(32) / 4
+    print("logprobs 2^24", flush=True)
+    got = gpu_logprobs(ws, x, bb.TYPE_F32, vocab, 1.0, np.array([[best[3]]], np.int32), 32)
+    y = x.astype(np.float64)
+    lse = 0.0 + np.log(np.exp(y).sum())
+    assert abs(got[1][0] - lse) < 2.0 ** -17 + 2.0 ** -22 * 40        # as check_logprobs counts it
+    assert np.array_equal(got[3][0], best[::-1]) and abs(got[0][0, 0] - (x[0, best[3]] - lse)) < 2.0 ** -16
+    lp = y - lse
+    assert abs(got[2][0] + (np.exp(lp) * lp).sum()) < 2.0 ** -17 * 20
+
+
 def test_logprobs_wanted_only(ws):
     rng = np.random.default_rng(1)
     x = rng.standard_normal((3, 700)).astype(np.float32)
@@ -383,6 +458,41 @@ def test_logprobs_wanted_only(ws):
     assert np.all(got[1] == 9.0) and np.all(got[2] == 9.0)
     full = gpu_logprobs(ws, x, bb.TYPE_F32, 700, 1.0, given, 3)
     assert np.array_equal(got[0], full[0]) and np.array_equal(got[3], full[3]) and np.array_equal(got[4], full[4])
+
+
+def test_two_streams_at_once():
+    """Two workspaces on two streams, their calls in flight together: the results of one after the other."""
+    syn = bb.synth()
+    st = [syn.pa_synth_stream_new() for _ in range(2)]
+    w = [bb.Workspace() for _ in range(2)]
+    loops = [Loop(21 + i, Q8, 128, 700, 12, vocab=50000) for i in range(2)]
+    print("two streams", flush=True)
+    try:
+        for l in loops:
+            l.append(l.d["x0"], l.d["pos0"], l.context, 0, None, None)
+            l.new_tree()
+        bb.device_sync()
+        want = []
+        for i, l in enumerate(loops):
+            l.step(w[i], st[i])
+            bb.device_sync()
+            want.append(l.outputs())
+        for _ in range(5):
+            for l in loops:
+                for k in ("o", "lse", "lp", "top"):
+                    l.d[k].upload(np.full(l.d[k].nbytes, 0x5a, np.uint8))
+            for _ in range(4):
+                for i, l in enumerate(loops):
+                    l.step(w[i], st[i])
+            bb.device_sync()
+            for l, o in zip(loops, want):
+                got = l.outputs()
+                assert all(np.array_equal(got[k], o[k]) for k in o)
+    finally:
+        for l in loops:
+            l.close()
+        for a in w:
+            a.close()
 
 
 # ---------------------------------------------------------------- row copies

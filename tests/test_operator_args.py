@@ -78,6 +78,8 @@ def logprobs(logits=P, type=bb.TYPE_F32, n_rows=3, vocab=1000, stride=1000, scal
     ("scale must be", dict(scale=-1.0)),
     ("scale must be", dict(scale=float("nan"))),
     ("scale must be", dict(scale=float("inf"))),
+    ("scale must be", dict(scale=1e-30)),
+    ("scale must be", dict(scale=1e30)),
     ("n_given must be", dict(n_given=-1)),
     ("n_given must be", dict(n_given=1025)),
     ("n_given must be", dict(n_top=33)),
