@@ -337,7 +337,7 @@ class PageTable:
     """The page table of `pages` as a call takes it, built once for a loop of calls (pages changed later need a new one)."""
 
     def __init__(self, pages: Pages):
-        self.n = len(pages.k)
+        self.pages, self.n = pages, len(pages.k)                     # (the buffers live as long as the table)
         m = max(self.n, 1)
         self.k, self.v = (C.c_void_p * m)(*pages.k), (C.c_void_p * m)(*pages.v)
         self.nkeys = (C.c_uint32 * m)(*pages.nkeys)
@@ -352,6 +352,7 @@ class LayerTable:
 
     def __init__(self, layers: list):
         self.layers, self.pages = len(layers), len(layers[0].k) if layers else 0
+        self.held = list(layers)                                     # (the buffers live as long as the table)
         if any(len(p.k) != self.pages or len(p.v) != self.pages for p in layers):
             raise PaHipError("LayerTable: every layer needs the same number of pages")
         m = max(self.layers * self.pages, 1)

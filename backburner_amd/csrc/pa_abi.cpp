@@ -1009,6 +1009,7 @@ extern "C" int pa_hip_append_rope(const pa_hip_shape * s, void * const * k_pages
     const char * fn = "pa_hip_append_rope";
     auto bad = [&](const std::string & why) { set_err(std::string(fn) + ": " + why); return -1; };
     if (!append_ok(fn, s, k_pages, v_pages, n_pages, page_keys, pos0, n)) return -1;
+    if (((uint64_t) pos0 + n) >> 32) return bad("positions must be below 2^32");
     if (!rope) return bad("null rope");
     if (rope->type > PA_TYPE_BF16) return bad("type must be 0 (f32), 1 (f16) or 2 (bf16)");
     if (rope->n_rot > s->hd || rope->n_rot % 2) return bad("n_rot must be even and at most hd");
@@ -1061,12 +1062,14 @@ extern "C" int pa_hip_copy_rows(const pa_hip_shape * s, int n_layers, const void
         }
     const uint64_t first = src_pos ? src_pos[0] : src_pos0, last = src_pos ? src_pos[n - 1] : (uint64_t) src_pos0 + n - 1;
     if (last >= (uint64_t) src_pages * page_keys) return bad("source positions past the last page");
+    if (last >> 32) return bad("positions must be below 2^32");
     const uint64_t dlast = (uint64_t) dst_pos0 + n - 1;
     if (dlast >= (uint64_t) dst_pages * page_keys) return bad("destination positions past the last page");
+    if (dlast >> 32) return bad("positions must be below 2^32");
     const uint32_t sp0 = (uint32_t) (first / page_keys), sp1 = (uint32_t) (last / page_keys);
     const uint32_t dp0 = dst_pos0 / page_keys, dp1 = (uint32_t) (dlast / page_keys);
     // every touched page, to see which are both: destinations by pointer in a table of open addressing, then the sources against it
-    bool in_place = false;
+    bool in_place = false, all_in_place = true;
     {
         struct Page { const void * p; uint64_t place; };
         static thread_local std::vector<Page> table;
@@ -1095,7 +1098,7 @@ extern "C" int pa_hip_copy_rows(const pa_hip_shape * s, int n_layers, const void
                     const void * x = (t ? src_v : src_k)[(size_t) l * src_pages + p];
                     if (!x) return bad("null source page " + std::to_string(p) + " of layer " + std::to_string(l));
                     const Page & at = find(x);
-                    if (!at.p) continue;
+                    if (!at.p) { all_in_place = false; continue; }
                     if (at.place != place(l, t, p)) return bad("a page is a source and, at another place, a destination");
                     in_place = true;
                 }
@@ -1104,7 +1107,8 @@ extern "C" int pa_hip_copy_rows(const pa_hip_shape * s, int n_layers, const void
     // in place positions only move down (they ascend, so the first says so for all)
     if (in_place && first < dst_pos0) return bad("rows moved in place must come from at or behind their destination");
     uint32_t i0 = 0;
-    if (in_place) while (i0 < n && from(i0) == dst_pos0 + i0) i0++;  // rows that stay
+    // rows that stay (not where tables share some of their pages, a fork's the full ones: the others take every row)
+    if (all_in_place) while (i0 < n && from(i0) == dst_pos0 + i0) i0++;
     const bool bulk = consecutive && (!in_place || first >= (uint64_t) dst_pos0 + n);
     CopyArgs a;
     a.rs = s->rs; a.row = s->nkv * s->hb;
@@ -1114,8 +1118,8 @@ extern "C" int pa_hip_copy_rows(const pa_hip_shape * s, int n_layers, const void
         uint32_t take = std::min(n - i0, page_keys - a.to0);
         if (bulk) {
             take = std::min(take, page_keys - a.from0);
-            // a launch's workgroups in 31 bits at any word size
-            take = std::min<uint64_t>(take, std::max<uint64_t>(1, (1ull << 40) / a.row));
+            // a launch's threads in 32 bits at any word size (4 words a thread)
+            take = std::min<uint64_t>(take, std::max<uint64_t>(1, (1ull << 33) / a.row));
         } else {
             take = std::min<uint32_t>(take, COPY_ROWS);
             uint32_t k = 0;

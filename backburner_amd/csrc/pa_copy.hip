@@ -53,7 +53,7 @@ template <typename W> static hipError_t launch_copy_w(bool list, const CopyArgs 
         const uint64_t words = (uint64_t) a.n * (a.row / sizeof(W));
         const uint32_t wpr = a.row / sizeof(W);
         const bool run = a.row == a.rs;
-        // (the host's checks keep a launch's words below 2^31 * 1024)
+        // (the host keeps a launch's words at 2^33 or fewer, its threads below 2^32)
         hipLaunchKernelGGL(copy_bulk_kernel<W>, dim3((uint32_t) ((words + 1023) / 1024), a.segs), dim3(256), 0, st, a, words,
                            run ? (uint32_t) 0 : wpr);
     }

@@ -246,7 +246,7 @@ typedef struct pa_hip_rope {
     uint64_t q_stride, k_stride, v_stride; /* elements from one token to the next; 0 = packed (heads * hd) */
 } pa_hip_rope;
 /* Q [n][nkv*rows/n][hd], K and V [n][nkv][hd] (device, 4-byte aligned; strides even for the 16-bit types), positions device
- * int32 [n], q_out 8-byte aligned; shape.rows a multiple of n. Q and q_out may both be NULL: keys and values only (rows is
+ * int32 [n], q_out 8-byte aligned and apart from the inputs; pos0 + n below 2^32; shape.rows a multiple of n. Q and q_out may both be NULL: keys and values only (rows is
  * then ignored). Pages, rs and hb as for pa_hip_append_f32. No counterpart in the reference (the fork's model graph does
  * this on the Mac). Returns 0 once enqueued, -1 on a bad argument (nothing enqueued). */
 int pa_hip_append_rope(const pa_hip_shape * shape, void * const * k_pages, void * const * v_pages, int n_pages,
@@ -257,8 +257,8 @@ int pa_hip_append_rope(const pa_hip_shape * shape, void * const * k_pages, void 
  * device pointers, layer-major, page p of a layer holding positions [p*page_keys, (p+1)*page_keys); src_pos: a
  * host array, strictly increasing. Two uses: the accepted path of a draft tree moved together (src and dst the same tables;
  * then src_pos[i] >= dst_pos0 + i, and each row arrives as it was before the call), and a fork filling its own copy of a
- * page. A page may appear as source and as destination only at the same place of its table, and as destination once. No
- * counterpart in the reference. Returns 0 once enqueued, -1 on a bad argument (nothing enqueued). */
+ * page. A page may appear as source and as destination only at the same place of its table (a fork's table may share its
+ * full pages), and as destination once. Positions are below 2^32. No counterpart in the reference. Returns 0 once enqueued, -1 on a bad argument (nothing enqueued). */
 int pa_hip_copy_rows(const pa_hip_shape * shape, int n_layers, const void * const * src_k, const void * const * src_v,
                      int src_pages, void * const * dst_k, void * const * dst_v, int dst_pages, uint32_t page_keys,
                      const uint32_t * src_pos, uint32_t src_pos0, uint32_t dst_pos0, uint32_t n, void * stream);

@@ -565,6 +565,30 @@ def test_copy_rows_fork(fmt, nkv, hd, pad, skew, layers, page_keys, at, to):
     a.buf.close(); b.buf.close()
 
 
+@pytest.mark.parametrize("layers,at,to,shared", [
+    (2, range(0, 120), 0, {0, 1}), (3, range(10, 64), 10, {0}), (2, [5, 6, 7, 60, 130], 5, {0, 2}), (2, list(range(50, 140)), 50, {1}),
+    (2, range(100, 140), 4, {0})])
+def test_copy_rows_into_a_table_that_shares_pages(layers, at, to, shared):
+    """A fork whose table holds its parent's own full pages (in every layer, and in one layer only) and copies of the others: rows of a
+    shared page move within it or stay, rows that stay in position still reach the pages of its own."""
+    print(f"copy shared={shared} layers={layers} n={len(at)} to={to}", flush=True)
+    rng = np.random.default_rng(len(at))
+    shape = bb.make_shape(2, 1, 128, Q8)
+    for where in (range(layers), range(1)):                          # the layers that share them
+        a, b = Cache(rng, layers, 3, 50, shape.rs), Cache(rng, layers, 3, 50, shape.rs)
+        share = lambda l, p: l in where and p in shared
+        table = [bb.Pages([(a if share(l, p) else b).table.k[3 * l + p] for p in range(3)],
+                          [(a if share(l, p) else b).table.v[3 * l + p] for p in range(3)], [50] * 3, []) for l in range(layers)]
+        want_a, want_b = a.bytes.copy(), b.bytes.copy()
+        for l in range(layers):
+            for i, f in enumerate(at):
+                (want_a if share(l, (to + i) // 50) else want_b)[l, :, to + i] = a.bytes[l, :, f]
+        bb.copy_rows(shape, a.table, bb.LayerTable(table), 50, at, to)
+        bb.device_sync()
+        assert np.array_equal(a.now(), want_a) and np.array_equal(b.now(), want_b)
+        a.buf.close(); b.buf.close()
+
+
 # ---------------------------------------------------------------- the loop
 class Loop:
     """A toy model of one layer whose next-token logits come from the tree attention's rows: append the tree's tokens, attend, score."""

@@ -123,6 +123,7 @@ def append(shape=None, counts=(64, 64), page_keys=64, pos0=60, rope_=None, Q=P, 
     ("page_keys", dict(page_keys=0)),
     ("past the last page", dict(pos0=125)),
     ("past the last page", dict(pos0=0xffffffff)),
+    ("positions must be below 2^32", dict(counts=(64, 64, 64), page_keys=1 << 31, pos0=(1 << 32) - 2)),
     ("null page", dict(k=None)),
     ("null page", dict(v=None)),
     ("type must be", dict(rope_=rope(type=3))),
@@ -206,6 +207,8 @@ def with_page(table, i, value, tensor="k"):
     ("at another place", lambda: bb.copy_rows(SHAPE, A, with_page(A, 1, A.k[0]), 64, [3, 5], 64)),
     ("at or behind their destination", lambda: bb.copy_rows(SHAPE, A, A, 64, [3, 5], 4)),
     ("at or behind their destination", lambda: bb.copy_rows(SHAPE, A, A, 64, range(0, 10), 1)),
+    ("positions must be below 2^32", lambda: bb.copy_rows(SHAPE, A, layers(3, 3), 1 << 31, range(0, 4), (1 << 32) - 3)),
+    ("positions must be below 2^32", lambda: bb.copy_rows(SHAPE, layers(3, 3), B, 1 << 31, range((1 << 32) - 5, (1 << 32) + 1), 0)),
     ("same number of layers", lambda: bb.copy_rows(SHAPE, A, layers(2, 2), 64, [0], 0)),
     ("same number of pages", lambda: bb.LayerTable([pages((64,)), pages((64, 64))])),
 ])
