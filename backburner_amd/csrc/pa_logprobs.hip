@@ -13,14 +13,16 @@
 //
 // The best n_top: a value is a 64-bit key (order of the value, ~id), so the largest key is the largest value and among equal
 // ones the lowest id. A wave collects candidates in LDS; sorted now and then (a key's place is the number of larger ones), their
-// n_top-th is a floor, and that a value lies below it (or below another wave's) is all that most values cost, without a barrier
-// in the loop. Before there is a floor, and where a lot of lanes pass it, the n_top-th largest of the lanes' maxima is one. At the
-// end the four waves' best are ranked.
+// n_top-th is a floor, and that a value lies below it (or below another wave's, or below the least of the four waves' (n_top / 4)-th
+// best) is all that most values cost, without a barrier in the loop. Before there is a floor, and where a lot of lanes pass it, the
+// n_top-th largest of the lanes' maxima is one. The values of the lanes that pass go through LDS, four lanes' at a time, one value per
+// lane. At the end the four waves' best are ranked.
 //
 // What bounds it: without alternatives the copy's rate (512 rows x 128,256 bf16 32 us, 4.1 TB/s; f32 51 us, 5.1 TB/s); with them the
-// vector instructions, about 5,600 per wave of 16 segments, half of them for the candidates (n_top 5 / 20: bf16 48 / 51 us, f32 59 /
-// 62). Candidates ranked by the whole workgroup at every segment with one took 99 us (n_top 20, bf16), kept sorted in the lanes by
-// insertion 60. A single row is latency: 5.6 us without, 10.8 with 5 alternatives of 151,936, in 38 workgroups.
+// vector instructions, about 4,800 per wave of 16 segments, half of them for the candidates (n_top 5 / 20: bf16 46 / 47 us, f32 57 /
+// 60). Candidates ranked by the whole workgroup at every segment with one took 99 us (n_top 20, bf16), kept sorted in the lanes by
+// insertion 60, one of each lane at a time without the shared floors 51. A single row is latency: 5.8 us without, 10.7 with 5
+// alternatives of 151,936, in 38 workgroups.
 #include "pa_attn.h"
 #include "pa_common.h"
 
@@ -29,7 +31,6 @@ namespace pa_hip {
 typedef unsigned long long lp_key;
 
 constexpr int LP_NV = 16, LP_SEG = 256 * LP_NV;
-constexpr int LP_MORE = 24;                                          // new candidates of a wave after which they are sorted for a new floor
 
 __device__ __forceinline__ uint32_t lp_order(float x) {              // NaN above everything, -0 == +0
     uint32_t u = __builtin_bit_cast(uint32_t, x);
@@ -115,7 +116,8 @@ template <> __device__ __forceinline__ float LpLoad<uint16_t>::value(uint16_t x)
 struct LpShared {
     __attribute__((aligned(16))) lp_key best[4][64];                 // per wave: scratch of a key per lane
     __attribute__((aligned(16))) lp_key tops[4][32];                 // the waves' best, 0 where there are fewer
-    __attribute__((aligned(16))) float fval[4];                      // the values of the waves' floors
+    __attribute__((aligned(16))) float fval[4], fquart[4];           // the values of the waves' floors, and of their (n_top / 4)-th best
+    uint8_t from[4][64];
     lp_key out[32];
     LpPart red[4];
     bool last;
@@ -136,7 +138,7 @@ __device__ __forceinline__ int lp_above(lp_key mine, lp_key * best) {
     best[threadIdx.x % 64] = mine;
     lp_wave_sync();
     int above = 0;
-    #pragma unroll 8
+    #pragma unroll 4
     for (int i = 0; i < 64; i += 2) {
         const pa_u4 x = *(const pa_u4 *) (best + i);
         above += (((lp_key) x.y << 32) | x.x) > mine;
@@ -252,7 +254,7 @@ __device__ __forceinline__ void lp_rank(LpTop & l, LpShared & sh) {
     __syncthreads();
 }
 
-template <typename T> __global__ __launch_bounds__(256) void logprob_kernel(const LogprobArgs a) {
+template <typename T> __global__ __launch_bounds__(256, 4) void logprob_kernel(const LogprobArgs a) {
     using L = LpLoad<T>;
     __shared__ LpShared sh;
     const int row = blockIdx.x / a.parts, w = blockIdx.x % a.parts, t = threadIdx.x;
@@ -270,10 +272,11 @@ template <typename T> __global__ __launch_bounds__(256) void logprob_kernel(cons
     if (a.parts == 1) given_load();
     LpPart p = {-INFINITY, 0.0f, 0.0f};
     extern __shared__ __attribute__((aligned(16))) lp_key lists[];   // [4][lp_room(n_top)], then [4][LP_NV / 4][64] x 4 floats
-    pa_f4 * vals = (pa_f4 *) (lists + 4 * lp_room(a.n_top)) + 64 * (LP_NV / 4) * (t / 64) + t % 64;
+    pa_f4 * vals = (pa_f4 *) (lists + 4 * lp_room(a.n_top)) + 64 * (LP_NV / 4) * (t / 64);
+    uint8_t * from = sh.from[t / 64];                                // the lanes whose values they are
     LpTop top;
     top.n = a.n_top; top.list = lists + lp_room(a.n_top) * (t / 64); top.best = sh.best[t / 64];
-    if (t < 4) sh.fval[t] = -INFINITY;
+    if (t < 4) sh.fval[t] = sh.fquart[t] = -INFINITY;
     if (a.n_top > 0) __syncthreads();
     pa_u4 r[L::NL];
     L::load(r, x + j0, min(j1 - j0, (uint32_t) LP_SEG));
@@ -298,9 +301,10 @@ template <typename T> __global__ __launch_bounds__(256) void logprob_kernel(cons
         }
         if (a.n_top == 0) continue;
         const bool any = L::at(0, t) < n, nan = p.s != p.s;             // (at(0): this thread's first value)
-        // what lies below another wave's floor is not wanted either (equal values may be: their ids can be lower here)
-        const pa_f4 fo = *(const volatile pa_f4 *) sh.fval;
-        float low = fmaxf(fmaxf(fo.x, fo.y), fmaxf(fo.z, fo.w));
+        // what lies below another wave's floor is not wanted either, nor what lies below the least of the four waves' (n / 4)-th best
+        // (equal values may be: their ids can be lower here)
+        const pa_f4 fo = *(const volatile pa_f4 *) sh.fval, fq = *(const volatile pa_f4 *) sh.fquart;
+        float low = fmaxf(fmaxf(fmaxf(fo.x, fo.y), fmaxf(fo.z, fo.w)), fminf(fminf(fq.x, fq.y), fminf(fq.z, fq.w)));
         bool hit = any && (nan || ((top.floor == 0 || mt > top.fval) && !(mt < low)));
         const int h = __builtin_popcountll(__ballot(hit));
         if (h == 0) continue;
@@ -312,29 +316,32 @@ template <typename T> __global__ __launch_bounds__(256) void logprob_kernel(cons
             low = ov > low ? ov : low;
         }
         low = fmaxf(low, top.fval);
-        // a lane's candidates (a NaN is one), one of each lane at a time: bits of their places, the values by LDS
-        uint32_t left = 0;
-        #pragma unroll
-        for (int i = LP_NV - 1; i >= 0; i--) left = left + left + (v[i] < low ? 0u : 1u);
-        left = hit ? left : 0;
-        #pragma unroll
-        for (int u = 0; u < LP_NV / 4; u++) vals[64 * u] = (pa_f4){v[4 * u], v[4 * u + 1], v[4 * u + 2], v[4 * u + 3]};
+        // the lanes' values by LDS, those of four lanes at a time, one per lane (a NaN is a candidate)
+        const unsigned long long who = __ballot(hit);
+        const int lanes = __builtin_popcountll(who), lane = t % 64;
+        if (hit) {
+            const int at = lp_below(who);
+            from[at] = lane;
+            #pragma unroll
+            for (int u = 0; u < LP_NV / 4; u++) vals[(LP_NV / 4) * at + u] = (pa_f4){v[4 * u], v[4 * u + 1], v[4 * u + 2], v[4 * u + 3]};
+        }
         lp_wave_sync();
-        for (;;) {
-            const bool more = __ballot(left != 0) != 0;
-            // sorted where the list might not take another 64, and after the segment for a new floor
-            if (more ? top.count + 64 > lp_room(top.n)
-                     : j + LP_SEG < j1 && top.count >= (top.floor == 0 ? top.n : top.n + LP_MORE)) {
-                top.sort();
-                if (t % 64 == 0) sh.fval[t / 64] = top.fval;
-            }
-            if (!more) break;
-            const uint32_t i = __builtin_ctz(left | 1u << 31) & (LP_NV - 1);
-            const float val = ((const float *) (vals + 64 * (i / 4)))[i % 4];
-            const uint32_t at = L::at(i, t);
-            const lp_key k = left != 0 && at < n ? lp_make_key(val, j + at) : 0;
-            left &= left - 1;
+        for (int l = lane / LP_NV; l - lane / LP_NV < lanes; l += 64 / LP_NV) {
+            if (top.count + 64 > lp_room(top.n)) top.sort();         // (the list might not take another 64)
+            const int s = min(l, 63);                                // (within the arrays)
+            const uint32_t at = L::at(lane % LP_NV, (uint32_t) (t - lane + from[s]));
+            const float val = ((const float *) vals)[LP_NV * s + lane % LP_NV];
+            const lp_key k = l < lanes && at < n && !(val < low) ? lp_make_key(val, j + at) : 0;
             top.push(k > top.floor, k);
+        }
+        // a new floor after n + 8 more (us, n_top 5 / 20 of 512 rows x 128,256 bf16: after 12 more 45.6 / 48.1, 24 47.7 / 47.2, 48 51.5 / 48.3)
+        if (j + LP_SEG < j1 && top.count >= (top.floor == 0 ? top.n : min(2 * top.n + 8, 64))) {
+            top.sort();
+            if (lane == 0) {
+                const int q = (top.n + 3) / 4 - 1;
+                sh.fval[t / 64] = top.fval;
+                sh.fquart[t / 64] = q < top.count ? lp_key_value(top.list[q]) : -INFINITY;
+            }
         }
     }
     // this part, then, by the row's last workgroup, all of them (one code for both: it runs once, and is fetched once)
