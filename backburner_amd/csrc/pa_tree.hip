@@ -9,12 +9,17 @@
 // matrix instruction multiplies a masked key's probability, zero, with whatever its value row holds, where infinities and NaN
 // become NaN. Here a value row that a row does not see is never read. At most 64 keys a row: vector work of a few instructions.
 //
-// W waves per row (1, 2, 4 or 8 by the number of slots), each with every W-th slot and all of its loads issued at once, against its
+// W waves per row (1, 2, 4 or 8, see launch_tree_w), each with every W-th slot and all of its loads issued at once, against its
 // own maximum; they meet once, through LDS. Lane l holds the dims (HD / 64) l .. of O. The row's first wave also takes the drafted
 // keys, only the ones that the row sees: four at a time, 16 lanes each, lane c with the dims (HD / 16) c .. of query, key and
 // value, so that a key's score is four lane swaps, and keys and values of 16 are in flight at once (a lane per key, whose row it reads
-// whole, and then a lane per dim took 5.0 us more of a call with 64 nodes of a tree, 24 of a chain).
+// whole, and then a lane per dim, took 1.6 us more for 64 nodes of a tree and 9.9 for a chain of 64, whose rows see 32 keys on average).
 //
+// What bounds it: reading the slots, and a chain of three memory round trips (mask, keys and values, slots): 4,096 rows x 16 slots (33.5
+// MB) and 64 nodes 11.8 us, 64 rows x 64 slots 5.4.
+//
+#include <algorithm>
+
 #include "pa_attn.h"
 #include "pa_common.h"
 
@@ -279,11 +284,17 @@ template <int HD, int FMT, int W> __global__ __launch_bounds__(W == 8 ? 512 : 25
     if (lane == 0) a.m.lse[r] = L == 0.0f ? -INFINITY : m * PA_LN2 + logf(L);
 }
 
+// Waves per row: with many slots more of them shorten a row's chain of loads, while the rows alone do not fill the CUs; with many rows
+// they only add a join. us of the kernel at head dim 128 with 1 / 2 / 4 / 8 waves, 8 drafted keys: 256 rows x 16 slots 5.6 / 6.2 / 5.6 / 5.7,
+// x 64 8.9 / 7.2 / 6.1 / 6.3, x 128 13.1 / 9.5 / 7.7 / 7.3; 1,024 rows x 16 slots 6.2 / 6.7 / 6.8 / 11.3, x 64 10.5 / 9.7 / 9.5 / 13.0;
+// 2,048 rows x 32 slots 9.9 / 10.3 / 13.0 / 21.6, x 64 14.6 / 13.4 / 16.8 / 24.1. Head dim 256, 128 rows x 16 slots 7.4 / 6.5 / 6.3 / 6.2, x 128
+// 22.8 / 10.0 / 8.3 / 7.8.
 template <int HD, int FMT> static void launch_tree_w(const TreeArgs & a, hipStream_t st) {
-    const uint32_t rows = a.m.nkv * a.m.rows;
-    if (a.m.n_slots <= 16) hipLaunchKernelGGL((tree_kernel<HD, FMT, 1>), dim3((rows + 3) / 4), dim3(256), 0, st, a);
-    else if (a.m.n_slots <= 32) hipLaunchKernelGGL((tree_kernel<HD, FMT, 2>), dim3((rows + 1) / 2), dim3(256), 0, st, a);
-    else if (a.m.n_slots <= 64) hipLaunchKernelGGL((tree_kernel<HD, FMT, 4>), dim3(rows), dim3(256), 0, st, a);
+    const uint32_t rows = a.m.nkv * a.m.rows, ns = a.m.n_slots;
+    const uint32_t w = std::min(ns > 64 ? 8u : ns > 16 ? 4u : 1u, rows <= 256 ? 8u : rows <= 1024 ? 4u : rows <= 2048 && ns > 32 ? 2u : 1u);
+    if (w == 1) hipLaunchKernelGGL((tree_kernel<HD, FMT, 1>), dim3((rows + 3) / 4), dim3(256), 0, st, a);
+    else if (w == 2) hipLaunchKernelGGL((tree_kernel<HD, FMT, 2>), dim3((rows + 1) / 2), dim3(256), 0, st, a);
+    else if (w == 4) hipLaunchKernelGGL((tree_kernel<HD, FMT, 4>), dim3(rows), dim3(256), 0, st, a);
     else hipLaunchKernelGGL((tree_kernel<HD, FMT, 8>), dim3(rows), dim3(512), 0, st, a);
 }
 

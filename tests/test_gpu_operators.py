@@ -182,6 +182,22 @@ def test_tree_padded_rows_and_split(ws, fmt, hd):
         ws.set_split(0, 0)
 
 
+@pytest.mark.parametrize("fmt,nkv,gqa,hd,nodes,context,wgs", [
+    (Q8, 3, 7, 128, 49, 4000, 288), (Q4, 3, 7, 128, 49, 4000, 288), (F16, 3, 7, 128, 49, 4000, 288), (Q8, 3, 7, 256, 49, 4000, 864),
+    (Q8, 1, 3, 128, 5, 9000, 100), (Q4, 2, 6, 256, 4, 9000, 200), (F16, 1, 8, 256, 3, 9000, 100),
+    (F16, 2, 5, 128, 9, 3000, 80), (Q4, 2, 5, 256, 9, 3000, 80), (Q8, 4, 8, 128, 64, 3000, 800)])
+def test_tree_rows_and_slots(ws, fmt, nkv, gqa, hd, nodes, context, wgs):
+    """Few and many rows with few and many split-K slots: every number of waves per row in the last step, odd numbers of rows among them."""
+    print(f"tree rows fmt={fmt} hd={hd} rows={nkv * gqa * nodes} context={context} workgroups={wgs}", flush=True)
+    rng, shape, K, V, Q = tree_case(hd + nodes + fmt, fmt, nkv, gqa, hd, nodes, context + nodes)
+    _, mask = plain.random_tree(rng, nodes)
+    ws.set_split(0, wgs)
+    try:
+        check_tree(shape, K, V, context + nodes, Q, nodes, mask, run_tree(ws, shape, K, V, [context + nodes], Q, nodes, mask))
+    finally:
+        ws.set_split(0, 0)
+
+
 def test_tree_own_stream_repeats(ws):
     """A stream of the caller's, and the same call again: the same bits."""
     rng, shape, K, V, Q = tree_case(31, Q8, 8, 8, 128, 20, 3000)
