@@ -1,7 +1,7 @@
 // pa_abi.cpp - the C ABI of libpa_hip.so (declared in include/phone_attn_hip.h): the reference's sme_* entry points
 // (phone-attn.h:63-71) and the device-resident engine path. Host C++ over the HIP runtime; all compute runs in the HIP
-// kernels (pa_decode.hip, pa_mma.hip, pa_attn.hip, pa_reply.hip, pa_ingest.hip, pa_accept.hip). There is no CPU
-// fallback: without a gfx950 device every call fails loudly. A workspace belongs to the device it was created on;
+// kernels (pa_decode.hip, pa_mma.hip, pa_mma256.hip, pa_merge.hip, pa_tree.hip, pa_reply.hip, pa_ingest.hip, pa_copy.hip,
+// pa_accept.hip, pa_logprobs.hip). There is no CPU fallback: without a gfx950 device every call fails loudly. A workspace belongs to the device it was created on;
 // calls that use it expect that device to be current.
 #include <hip/hip_runtime.h>
 
@@ -493,6 +493,11 @@ bool mma_wide256(const pa_hip_shape * s, const uint32_t * nkeys, int n_pages) {
     return wide < narrow;
 }
 
+// Slots from one row's first to the next row's. A wave writes its 32 rows' shares of one slot together; at a multiple of 8 slots (4 or 8 KB)
+// they fall into few of the L2's sets and leave it in parts: 208 rows x 8 heads x 32 slots wrote 58 MB of the 27 that they are, at an
+// odd distance 34 (33,333 q4_0 keys, a call of 26 nodes 77.1 us and 71.0).
+uint64_t tree_slot_stride(uint64_t n_slots) { return n_slots + (n_slots % 8 == 0 ? 1 : 0); }
+
 // the matrix-core kernels, over chunks of 32-key tiles: mma_kernel (row blocks of 32*NW rows) for every head-dim-128 call
 // that attn_decode does not take and for long head-dim-256 contexts above 64 rows; mma256_kernel (row blocks of 64 rows) for
 // the other head-dim-256 calls
@@ -551,7 +556,8 @@ int attn_mma(Call & cx, const pa_hip_shape * s, const void * const * k_pages, co
         });
         if (room > rows_per_slot) cx.reserve(room, s->hd, st);
     }
-    if (!direct && !cx.slots(n_slots * rows_per_slot, s->hd, st)) return -1;
+    const uint64_t stride = cx.tree ? tree_slot_stride(n_slots) : n_slots;   // slots from a row's first to the next row's
+    if (!direct && !cx.slots(stride * rows_per_slot, s->hd, st)) return -1;
     uint32_t li = 0, slot0 = 0;
     bool ok = true;
     for_launches(nkeys, n_pages, [&](int p0, int np, uint64_t tiles, uint64_t) {
@@ -563,7 +569,7 @@ int attn_mma(Call & cx, const pa_hip_shape * s, const void * const * k_pages, co
         a.n_chunks = nch; a.chunk = tpc;
         a.n_items = nch * units;
         a.rs = s->rs; a.hb = s->hb; a.nkv = s->nkv; a.rows = s->rows; a.qr = qr; a.nrb = nrb; a.slot0 = slot0;
-        a.slots = (uint32_t) n_slots;
+        a.slots = (uint32_t) stride;
         a.qmode = s->qmode; a.fused = direct ? 1u : 0u; a.scale = s->scale; a.s_mul = 1.4426950408889634f;
         a.q = Q; a.po = cx.po; a.pml = cx.pml; a.O = O; a.m = m; a.l = l;
         // Fewer chunks than the round hold more tiles each, and the fp16 rounding of P costs more there: a chunk's probabilities are
@@ -591,7 +597,7 @@ int attn_mma(Call & cx, const pa_hip_shape * s, const void * const * k_pages, co
     MergeArgs ma;
     ma.po = cx.po; ma.pml = cx.pml; ma.O = O; ma.m = m; ma.l = l;
     ma.n_slots = (uint32_t) n_slots; ma.nkv = s->nkv; ma.qr = qr; ma.rows = s->rows;
-    ma.sst = 1; ma.rst = n_slots;
+    ma.sst = 1; ma.rst = stride;
     return cx.merge(ma, (int) s->hd, st) ? 0 : -1;
 }
 

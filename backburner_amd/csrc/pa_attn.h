@@ -63,8 +63,8 @@ struct TreeArgs {
 hipError_t launch_tree(int hd, int fmt, const TreeArgs & a, hipStream_t st);
 
 hipError_t launch_merge(int hd, const MergeArgs & a, hipStream_t st);
-// px: probabilities kept to more bits than one fp16 rounding (ggml's query rounding at the 16-row and 32-row kernels' head dims only;
-// see the kernels)
+// px: probabilities kept to more bits than one fp16 rounding (pa_hip_attn_tree; PA_QMODE_GGML only, and at head dim 256 the 16-row
+// kernel only)
 hipError_t launch_decode(int fmt, bool px, const AttnArgs & a, uint32_t grid, hipStream_t st, hipEvent_t ev0 = nullptr,
                          hipEvent_t ev1 = nullptr);
 hipError_t launch_mma(int hd, int fmt, int nw, bool skip, int streams, bool px, const AttnArgs & a, uint32_t grid, hipStream_t st,
