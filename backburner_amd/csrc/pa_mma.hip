@@ -178,8 +178,8 @@ __device__ __forceinline__ void mm_write_out(const AttnArgs & a, const mm_f16 (&
 // rounded once, P enters as the fp16 pair (p, p - fp16(p)), two MFMAs instead of one; over f16 V, exact in fp16, as one; and
 // the row sum adds the fp32 probabilities. At head dim 128 the exact dots' scale pairs are held 2^6 times larger (QS in mm_prep_qi8:
 // the usual factors, fp16(d) / sqrt(128) of queries of size 1, lie at 2^-9, where lo falls into the subnormals and a score is off
-// by 1e-5, which a log-sum-exp shows). The second MFMA and the split cost about a quarter: 512 rows x 8 heads x 98,304 q8_0 keys, a
-// whole call with its join, 348 us, 269 without (call after call); a reply's error against 64 bits 2.9e-4 (2-norm; fp16 itself 2.1e-4), its log-sum-exp's 4e-8.
+// by 1e-5, which a log-sum-exp shows). The second MFMA and the split cost about a fifth: 512 rows x 8 heads x 98,304 q8_0 keys, a
+// whole call with its join, 329 us, 270 without (call after call); a reply's error against 64 bits 2.9e-4 (2-norm; fp16 itself 2.1e-4), its log-sum-exp's 4e-8.
 template <int HD, int FMT, int NW, bool SKIP, bool EX, int NS = 1, bool PX = false>
 __global__ __launch_bounds__(64 * NW, 8 / NW) void mma_kernel(const AttnArgs a) {   // 2 waves per SIMD
     static_assert(!EX || FMT != 0, "the exact block dots take quantized K");
@@ -380,6 +380,11 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void mma_kernel(const AttnArgs a) 
         }
         __builtin_amdgcn_sched_barrier(0);
     };
+    // LATE: waves 4-7 pass the step's barrier before their PV instead of after it (V^T is in registers by then, so the stage is read out),
+    // and their PV runs beside the QK and the softmax of the older wave of their SIMD. us with all waves at the end and so, 32,768 keys x
+    // 8 heads: 512 rows q8_0 142 / 138, q4_0 148 / 144, f16 94.8 / 96.1; with waves that only stage, 160 rows x 65,536 q8_0 114 / 117, f16
+    // 75.0 / 71.0. The older waves late instead: 512 rows 144, 147.
+    constexpr bool LATE = PX && NW == 8 && HD == 128 && EX != SKIP;
     // one tile's matrix work on LDS stage `stage` (nvalid keys)
     auto compute = [&](int stage, int nvalid) {
         const char * Kt = smem + (stage * NS + sx) * G::STAGE;
@@ -515,11 +520,21 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void mma_kernel(const AttnArgs a) 
         }
 
         // ---- O^T += V^T P^T
-        #pragma unroll
-        for (int i = 0; i < 2 * NBLK; i++) {
-            O[i >> 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va[i % VA], P[i & 1], O[i >> 1], 0, 0, 0);
-            if constexpr (PX && FMT != 0) O[i >> 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va[i % VA], Pl[i & 1], O[i >> 1], 0, 0, 0);
-            if (i + VA < 2 * NBLK) v_read(i + VA);
+        if constexpr (PX && HD == 128) {                             // (all of V^T is in registers)
+            if constexpr (LATE) { if (wave >= NW / 2) mm_lds_barrier(); }
+            #pragma unroll
+            for (int i = 0; i < (FMT != 0 ? 4 : 2); i++)             // dim blocks one after the other: no MFMA waits for the one before
+                #pragma unroll
+                for (int db = 0; db < NBLK; db++) {
+                    const int mi = FMT != 0 ? i / 2 : i;
+                    O[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va[2 * db + mi], FMT != 0 && (i & 1) ? Pl[mi] : P[mi], O[db], 0, 0, 0);
+                }
+        } else {
+            #pragma unroll
+            for (int i = 0; i < 2 * NBLK; i++) {
+                O[i >> 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va[i % VA], P[i & 1], O[i >> 1], 0, 0, 0);
+                if (i + VA < 2 * NBLK) v_read(i + VA);
+            }
         }
     };
     // one tile step; Rn holds tile t + 1's raw bytes
@@ -547,7 +562,8 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void mma_kernel(const AttnArgs a) 
         store_tile(Rn, stage ^ 1);
         load_tile(Rn, t + 1 + PF);
         if (clive) compute(stage, nvalid);
-        mm_lds_barrier();                                            // this stage is free; the next one is written
+        if constexpr (LATE) { if (!(wave >= NW / 2 && clive)) mm_lds_barrier(); }
+        else mm_lds_barrier();                                       // this stage is free; the next one is written
     };
     const uint32_t nsteps = (ntiles + NS - 1) / NS;
     uint32_t t = 0;                                                  // step t + 1's tiles are in R((t + 1) % PF)
