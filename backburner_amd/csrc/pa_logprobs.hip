@@ -133,17 +133,19 @@ __device__ __forceinline__ lp_key lp_lane(lp_key k, int lane) {
     return ((lp_key) (uint32_t) __builtin_amdgcn_readlane((int) (k >> 32), lane) << 32) | (uint32_t) __builtin_amdgcn_readlane((int) k, lane);
 }
 
-// the number of the wave's 64 keys above this lane's
-__device__ __forceinline__ int lp_above(lp_key mine, lp_key * best) {
+// the number of the first n lanes' keys above this lane's (the others' are 0)
+__device__ __forceinline__ int lp_above(lp_key mine, lp_key * best, int n) {
     best[threadIdx.x % 64] = mine;
     lp_wave_sync();
     int above = 0;
-    #pragma unroll 4
-    for (int i = 0; i < 64; i += 2) {
-        const pa_u4 x = *(const pa_u4 *) (best + i);
-        above += (((lp_key) x.y << 32) | x.x) > mine;
-        above += (((lp_key) x.w << 32) | x.z) > mine;
-    }
+    #pragma unroll 1
+    for (int i = 0; i < n; i += 8)
+        #pragma unroll
+        for (int k = 0; k < 8; k += 2) {
+            const pa_u4 x = *(const pa_u4 *) (best + i + k);
+            above += (((lp_key) x.y << 32) | x.x) > mine;
+            above += (((lp_key) x.w << 32) | x.z) > mine;
+        }
     lp_wave_sync();
     return above;
 }
@@ -194,7 +196,7 @@ struct LpTop {
             const int had = count;
             lp_key mine = 0;
             for (int i = lane; i < had; i += 64) mine = list[i] > mine ? list[i] : mine;
-            const unsigned long long who = __ballot(lp_above(mine, best) == n - 1 && mine != 0);
+            const unsigned long long who = __ballot(lp_above(mine, best, 64) == n - 1 && mine != 0);
             const lp_key fl = who ? lp_lane(mine, __builtin_ctzll(who)) : 1;
             count = 0;
             for (int i = 0; i < had; i += 64) {                      // (no write passes what has been read)
@@ -206,7 +208,7 @@ struct LpTop {
         }
         if (count <= 64) {                                           // one key per lane, its place the number of larger ones
             const lp_key k = lane < count ? list[lane] : 0;
-            const int place = lp_above(k, best);
+            const int place = lp_above(k, best, count);
             if (k && place < n) list[place] = k;
             count = min(count, n);
         } else {                                                     // rare (the best in few lanes): one after the other, sorted in
