@@ -19,9 +19,9 @@
 // lane. At the end the four waves' best are ranked.
 //
 // What bounds it: without alternatives the copy's rate (512 rows x 128,256 bf16 32 us, 4.1 TB/s; f32 51 us, 5.1 TB/s); with them the
-// vector instructions, about 4,800 per wave of 16 segments, half of them for the candidates (n_top 5 / 20: bf16 46 / 47 us, f32 57 /
-// 60). Candidates ranked by the whole workgroup at every segment with one took 99 us (n_top 20, bf16), kept sorted in the lanes by
-// insertion 60, one of each lane at a time without the shared floors 51. A single row is latency: 5.8 us without, 10.7 with 5
+// vector instructions, about 4,600 per wave of 16 segments, half of them for the candidates (n_top 5 / 20: bf16 42 / 45 us, f32 54 /
+// 58). Candidates ranked by the whole workgroup at every segment with one took 99 us (n_top 20, bf16), kept sorted in the lanes by
+// insertion 60, one of each lane at a time without the shared floors 51. A single row is latency: 5.7 us without, 10.2 with 5
 // alternatives of 151,936, in 38 workgroups.
 #include "pa_attn.h"
 #include "pa_common.h"
@@ -256,6 +256,7 @@ __device__ __forceinline__ void lp_rank(LpTop & l, LpShared & sh) {
     __syncthreads();
 }
 
+// (four workgroups per CU, the whole launch at once: 132 registers would leave three, f32 512 rows 79 us instead of 58)
 template <typename T> __global__ __launch_bounds__(256, 4) void logprob_kernel(const LogprobArgs a) {
     using L = LpLoad<T>;
     __shared__ LpShared sh;
@@ -336,7 +337,8 @@ template <typename T> __global__ __launch_bounds__(256, 4) void logprob_kernel(c
             const lp_key k = l < lanes && at < n && !(val < low) ? lp_make_key(val, j + at) : 0;
             top.push(k > top.floor, k);
         }
-        // a new floor after n + 8 more (us, n_top 5 / 20 of 512 rows x 128,256 bf16: after 12 more 45.6 / 48.1, 24 47.7 / 47.2, 48 51.5 / 48.3)
+        // a new floor after n + 8 more (us, n_top 5 / 20 of 512 rows x 128,256 bf16, of an earlier form: after 12 more 45.6 / 48.1, 24 47.7 / 47.2,
+        // 48 51.5 / 48.3)
         if (j + LP_SEG < j1 && top.count >= (top.floor == 0 ? top.n : min(2 * top.n + 8, 64))) {
             top.sort();
             if (lane == 0) {
