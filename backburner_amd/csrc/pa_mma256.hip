@@ -59,7 +59,8 @@ __device__ __forceinline__ float m2_sum16(float v) {    // sum over lanes l and 
 // EX: exact block dots in ggml's query rounding (quantized K only). WPS: waves per SIMD the registers are sized for.
 // Instantiated at head dim 256; at 128 (three waves per SIMD, 167 VGPRs) the 16-row waves measured slower than the
 // 32-row mma_kernel on verify (157 against 111 us), each wave reading the whole K / V^T tile from LDS.
-// PX: probabilities to more than one fp16 rounding, as in mma_kernel.
+// PX: probabilities to more than one fp16 rounding, as in mma_kernel. With SKIP one tile in flight and K read four steps ahead (us, 48 rows
+// x 4 heads x 65,536 q8_0 keys with the join 72.5 / 69.4, q4_0 71.4 / 68.4, 6 rows 56.5 / 51.4).
 template <int HD, int FMT, bool SKIP, bool EX, int WPS, bool PX = false>
 __global__ __launch_bounds__(256, WPS) void mma256_kernel(const AttnArgs a) {
     static_assert(!EX || FMT != 0, "exact block dots need quantized K");
@@ -67,7 +68,7 @@ __global__ __launch_bounds__(256, WPS) void mma256_kernel(const AttnArgs a) {
     constexpr int NBLK = G2::NBLK, M2_KST = G2::KST, M2_VST = G2::VST, M2_KT = G2::KT, M2_VT = G2::VT;
     constexpr int M2_STAGE = G2::STAGE;
     // NB tiles' raw bytes are in flight while a tile is computed (a ring of NB register buffers)
-    constexpr int NT = 256, NB = EX && !SKIP ? 1 : 2;                // (full row blocks of EX: one, the registers of two spill)
+    constexpr int NT = 256, NB = EX && (!SKIP || PX) ? 1 : 2;      // (full row blocks of EX: one, the registers of two spill)
     constexpr int UPT = 128 * NBLK / NT;                             // staging units per thread (128 NBLK per tile)
     __shared__ __attribute__((aligned(16))) char smem[2 * M2_STAGE];
 
@@ -252,7 +253,7 @@ __global__ __launch_bounds__(256, WPS) void mma256_kernel(const AttnArgs a) {
         __builtin_amdgcn_s_waitcnt(0xc07f);                          // lgkmcnt(0): the stores and any scalar load done
         // ---- S^T = K Q'^T: the two key halves' chains interleaved, K read four steps ahead
         pa_f4 S[2] = {(pa_f4){}, (pa_f4){}};
-        constexpr int KA = EX ? 1 : (NBLK < 4 ? NBLK : 4);           // K read KA steps ahead (EX holds more registers)
+        constexpr int KA = EX ? (PX && SKIP ? 4 : 1) : (NBLK < 4 ? NBLK : 4);   // K read KA steps ahead (EX holds more registers)
         mm_h8 kf[2][KA];
         auto k_read = [&](int s) {
             #pragma unroll
@@ -355,13 +356,18 @@ __global__ __launch_bounds__(256, WPS) void mma256_kernel(const AttnArgs a) {
         // ---- O^T += V^T P^T per 16-dim block: lane (g, L) of a transposing read addresses key 16 r + 4 g + L / 4,
         // dims 16 db + 4 (L % 4) .. +3; lane (g, s) then holds dim 16 db + s of keys 16 r + 4 g + j (j < 4)
         const char * vrow = Vt + (4 * g + (n >> 2)) * M2_VST + 2 * 4 * (n & 3);
+        mm_h8 vp;
         #pragma unroll
         for (int db = 0; db < HD / 16; db++) {
             const pa_h4 x0 = __builtin_bit_cast(pa_h4, __builtin_amdgcn_ds_read_tr16_b64_v4f16((MM_LDS mm_tr4 *) (vrow + 32 * db)));
             const pa_h4 x1 = __builtin_bit_cast(pa_h4, __builtin_amdgcn_ds_read_tr16_b64_v4f16((MM_LDS mm_tr4 *) (vrow + 16 * M2_VST + 32 * db)));
             const mm_h8 va = __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7);
             O[db] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, P, O[db], 0, 0, 0);
-            if constexpr (PX && FMT != 0) O[db] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, Pl, O[db], 0, 0, 0);
+            if constexpr (PX && FMT != 0) {                          // (a block behind: no MFMA waits for the one before)
+                if (db > 0) O[db - 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vp, Pl, O[db - 1], 0, 0, 0);
+                vp = va;
+                if (db == HD / 16 - 1) O[db] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vp, Pl, O[db], 0, 0, 0);
+            }
         }
     };
     auto step = [&](uint32_t t, int r) {
