@@ -816,6 +816,7 @@ extern "C" int pa_hip_attn_tree(pa_hip_ws * ws, const pa_hip_shape * s, const vo
     if (n_nodes < 1 || n_nodes > 64) return bad("n_nodes must be 1..64");
     if (s->rows % n_nodes) return bad("rows must be a multiple of n_nodes");
     if (s->qmode != PA_QMODE_GGML) return bad("qmode must be 0 (ggml)");
+    if (!(s->scale >= 0.0f) || !std::isfinite(s->scale)) return bad("scale must be finite and not negative");
     if ((uint64_t) s->nkv * s->rows > (1ull << 24)) return bad("more than 2^24 rows");
     if (!mask || !Q || !Oh || !lse) return bad("null mask/Q/Oh/lse");
     if (!aligned(mask, 8) || !aligned(Q, 4) || !aligned(Oh, 8) || !aligned(lse, 4))

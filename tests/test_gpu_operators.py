@@ -352,6 +352,26 @@ def test_append_rope_keys_only_and_values_of_zero():
         assert np.array_equal(got.reshape(4, -1)[1:], rows) and np.all(got.reshape(4, -1)[0] == 0xa5)
 
 
+def test_append_rope_many_tokens_and_positions_before_zero():
+    """More tokens than a launch takes (65,535), over more pages than one names (16); negative positions turn the other way."""
+    nkv, gqa, hd, n, pos0, page_keys = 1, 1, 128, 70000, 11, 2048
+    rng = np.random.default_rng(5)
+    x = rng.standard_normal((n, 3 * hd)).astype(np.float32)
+    pos = rng.integers(-1000, 140000, n)
+    freq = (1e4 ** (-2.0 * np.arange(64) / 128)).astype(np.float32)
+    w = [(1.0 + 0.3 * rng.standard_normal(hd)).astype(np.float32) for _ in range(2)]
+    shape = bb.make_shape(nkv, gqa * n, hd, Q4)
+    n_pages = (pos0 + n + page_keys - 1) // page_keys
+    q, k, v = gpu_append(shape, n_pages, page_keys, pos0, {"w": w, "freq": freq, "eps": 1e-6, "n_rot": 128, "interleaved": False}, x, pos, n, gqa,
+                         bb.TYPE_F32)
+    vals = x.reshape(n, 3, hd)
+    wq, wk = (plain.norm_rope(vals[:, i:i + 1], w[i], 1e-6, freq, pos, 128, False) for i in (0, 1))
+    assert np.all(np.abs(q[0, 0] - wq[:, 0]) <= 2.0 ** -24 * np.abs(wq[:, 0]) + 2.0 ** -49 * np.abs(wq).max(2))
+    for got, ref in ((k, wk.astype(np.float32)), (v, vals[:, 2:])):
+        rows = orc.rows_from_f32(Q4, np.ascontiguousarray(ref), shape.rs, shape.hb).reshape(n, -1)
+        assert np.array_equal(got.reshape(-1, shape.rs)[pos0:pos0 + n], rows)
+
+
 # ---------------------------------------------------------------- log probabilities
 def gpu_logprobs(ws, raw, type, vocab, scale, given, n_top, stream=None, wanted=True):
     rows, stride = raw.shape
@@ -410,6 +430,25 @@ def test_logprobs(ws, type, rows, vocab, stride, n_given, n_top):
         given[0, 0], given[-1, 1] = -1, vocab
     for scale in (1.0, 0.7):
         check_logprobs(vals[:, :vocab], scale, given, n_top, gpu_logprobs(ws, raw, type, vocab, scale, given, n_top))
+
+
+@pytest.mark.parametrize("type", [bb.TYPE_F32, bb.TYPE_BF16])
+@pytest.mark.parametrize("n_top", [1, 5, 32])
+def test_logprobs_whole_rows_of_a_workgroup(ws, type, n_top):
+    """So many rows that a workgroup streams a whole one: values in ascending, descending and random order, with few different values
+    (ties, the lowest id first), ever larger towards one lane's places, and the best ones at the row's end."""
+    rows, vocab = 1026, 9001
+    print(f"logprobs whole rows type={type} top={n_top}", flush=True)
+    rng = np.random.default_rng(n_top)
+    x = (rng.standard_normal((rows, vocab)) * 2.0).astype(np.float32)
+    up = np.linspace(-9.0, 9.0, vocab, dtype=np.float32)
+    x[0::6], x[1::6] = up, up[::-1]
+    x[2::6] = rng.integers(-3, 4, x[2::6].shape)
+    x[3::6, 5::1024] += np.arange(len(range(5, vocab, 1024)), dtype=np.float32) + 9.0
+    x[4::6, -40:] += 12.0
+    raw, vals = to_type(x, type)
+    given = rng.integers(0, vocab, (rows, 1)).astype(np.int32)
+    check_logprobs(vals, 1.0, given, n_top, gpu_logprobs(ws, raw, type, vocab, 1.0, given, n_top))
 
 
 @pytest.mark.parametrize("vocab", [40, 5000, 70000])

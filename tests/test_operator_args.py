@@ -35,6 +35,7 @@ def tree(shape=None, counts=(100, 50), n_nodes=4, mask=P, Q=P, Oh=P, lse=P, k=P,
     ("n_nodes must be 1..64", dict(n_nodes=65, shape=bb.make_shape(2, 65, 128, bb.FMT_Q8_0))),
     ("multiple of n_nodes", dict(n_nodes=5)),
     ("qmode must be 0", dict(shape=bb.make_shape(2, 16, 128, bb.FMT_Q8_0, bb.QMODE_F16))),
+    *(("scale must be finite", dict(shape=bb.Shape(2, 16, 128, 1, 272, 136, 0, x))) for x in (-0.1, float("nan"), float("inf"))),
     ("hd must be 128 or 256", dict(shape=bb.make_shape(2, 16, 64, bb.FMT_Q8_0))),
     ("fmt must be", dict(shape=bb.Shape(2, 16, 128, 3, 272, 136, 0, 0.1))),
     ("nkv and rows", dict(shape=bb.make_shape(0, 16, 128, bb.FMT_Q8_0))),
