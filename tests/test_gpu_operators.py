@@ -182,6 +182,33 @@ def test_tree_padded_rows_and_split(ws, fmt, hd):
         ws.set_split(0, 0)
 
 
+def with_head_gaps(rows, nkv, hb, gap, fill):
+    """[n][nkv * hb] bytes with `gap` bytes of `fill` behind every head."""
+    h = rows.reshape(-1, nkv, hb)
+    return np.concatenate([h, np.full((len(h), nkv, gap), fill, np.uint8)], 2).reshape(len(h), nkv * (hb + gap))
+
+
+@pytest.mark.parametrize("fmt", [Q8, Q4, F16])
+@pytest.mark.parametrize("hd", [128, 256])
+def test_heads_with_gaps(ws, fmt, hd):
+    """Heads further apart than their bytes (hb): the same tree attention bit for bit as over packed ones, whatever lies between, and the
+    same appended heads, with nothing written between."""
+    nkv, gqa, nodes, context, gap = 2, 4, 5, 300, 12
+    rng, shape, K, V, Q = tree_case(700 + hd + fmt, fmt, nkv, gqa, hd, nodes, context + nodes)
+    _, mask = plain.random_tree(rng, nodes)
+    wide = bb.Shape(nkv, shape.rows, hd, fmt, nkv * (shape.hb + gap), shape.hb + gap, 0, shape.scale)
+    want = run_tree(ws, shape, K, V, [context + nodes], Q, nodes, mask)
+    got = run_tree(ws, wide, *(with_head_gaps(x, nkv, shape.hb, gap, 0x7e).reshape(-1) for x in (K, V)), [context + nodes], Q, nodes, mask)
+    assert np.array_equal(got[0], want[0]) and np.array_equal(got[1], want[1])
+    x = rng.standard_normal((9, (nkv * gqa + 2 * nkv) * hd)).astype(np.float32)
+    args = {"w": [None, None], "freq": np.ones(hd // 2, np.float32), "eps": 0.0, "n_rot": hd, "interleaved": False}
+    packed, spaced = (gpu_append(bb.Shape(nkv, gqa * 9, hd, fmt, s.rs, s.hb, 0, 1.0), 2, 8, 3, args, x, np.arange(9), 9, gqa, bb.TYPE_F32)
+                      for s in (shape, wide))
+    assert np.array_equal(packed[0], spaced[0])
+    for p, s in zip(packed[1:], spaced[1:]):
+        assert np.array_equal(with_head_gaps(p, nkv, shape.hb, gap, 0xa5), s.reshape(-1, wide.rs))
+
+
 @pytest.mark.parametrize("fmt,nkv,gqa,hd,nodes,context,wgs", [
     (Q8, 3, 7, 128, 49, 4000, 288), (Q4, 3, 7, 128, 49, 4000, 288), (F16, 3, 7, 128, 49, 4000, 288), (Q8, 3, 7, 256, 49, 4000, 864),
     (Q8, 1, 3, 128, 5, 9000, 100), (Q4, 2, 6, 256, 4, 9000, 200), (F16, 1, 8, 256, 3, 9000, 100),
