@@ -871,8 +871,8 @@ extern "C" int pa_hip_logprobs(pa_hip_ws * ws, const void * logits, int type, in
     LogprobArgs a;
     const int64_t segs = (vocab + 4095) / 4096;
     // Workgroups of a row: 1,024 in all, four per CU (what is resident at once); more only add ends, fewer leave loads unhidden. us at
-    // 512 / 1,024 / 2,048 in all, 20 alternatives: 512 rows x 128,256 f32 68.5 / 63.1 / 77.0, bf16 54.6 / 58.3 / 71.1, 27 rows x
-    // 151,936 f32 21.5 / 21.1 / 25.4 (of an earlier form of the kernel).
+    // 512 / 1,024 / 1,536 in all, 20 alternatives: 512 rows x 128,256 bf16 48.5 / 45.0 / 58.4, f32 55.3 / 57.7 / 67.7, 27 rows x
+    // 151,936 f32 19.1 / 19.5 / 23.8. A single row takes a segment each (10.1; two each 12.2).
     int64_t parts = std::min<int64_t>({segs, LP_MAX_PARTS, std::max<int64_t>(1, 1024 / n_rows)});
     const int64_t per = (segs + parts - 1) / parts;
     parts = (segs + per - 1) / per;
