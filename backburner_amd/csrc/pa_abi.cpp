@@ -1058,7 +1058,7 @@ extern "C" int pa_hip_copy_rows(const pa_hip_shape * s, int n_layers, const void
     auto bad = [&](const std::string & why) { set_err("pa_hip_copy_rows: " + why); return -1; };
     if (!s || s->nkv == 0 || s->hb == 0 || (uint64_t) s->rs < (uint64_t) s->nkv * s->hb) return bad("bad shape");
     if (s->rs >= (1u << 26)) return bad("rs must be below 2^26 bytes");
-    if (n_layers < 0 || src_pages < 0 || dst_pages < 0 || page_keys == 0) return bad("bad layer or page count");
+    if (n_layers < 0 || n_layers > (1 << 20) || src_pages < 0 || dst_pages < 0 || page_keys == 0) return bad("bad layer or page count");
     if (n == 0 || n_layers == 0) return 0;
     if (!src_k || !src_v || !dst_k || !dst_v) return bad("null page table");
     bool consecutive = true;

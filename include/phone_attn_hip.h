@@ -252,7 +252,7 @@ typedef struct pa_hip_rope {
 int pa_hip_append_rope(const pa_hip_shape * shape, void * const * k_pages, void * const * v_pages, int n_pages,
                        uint32_t page_keys, uint32_t pos0, const pa_hip_rope * rope, const void * Q, const void * K,
                        const void * V, const int32_t * positions, uint32_t n, float * q_out, void * stream);
-/* Copies n rows (the nkv*hb bytes of the shape's row format) of K and of V in every one of n_layers layers: the row at position
+/* Copies n rows (the nkv*hb bytes of the shape's row format) of K and of V in every one of n_layers (0 .. 2^20) layers: the row at position
  * src_pos[i] (src_pos NULL: src_pos0 + i) to position dst_pos0 + i. src_k .. dst_v: host arrays of n_layers * src_pages (dst_pages)
  * device pointers, layer-major, page p of a layer holding positions [p*page_keys, (p+1)*page_keys); src_pos: a
  * host array, strictly increasing. Two uses: the accepted path of a draft tree moved together (src and dst the same tables;

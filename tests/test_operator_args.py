@@ -222,6 +222,11 @@ def test_copy_rows_nothing_to_do():
     bb.copy_rows(SHAPE, A, A, 64, [7, 8, 9], 7)                      # every row stays where it is: nothing is enqueued
 
 
+def test_copy_rows_too_many_layers():
+    assert bb.lib().pa_hip_copy_rows(C.byref(SHAPE), (1 << 20) + 1, A.k, A.v, 2, B.k, B.v, 2, 64, None, 0, 0, 5, None) == -1
+    assert "bad layer" in bb.last_error()
+
+
 def test_copy_rows_null_tables():
     z = C.POINTER(C.c_void_p)()
     for t in range(4):
